@@ -423,6 +423,88 @@ int sedmi_confusion_counts(const float *p, const float *labels, int64_t n_rows, 
                            float thr, int apply_sigmoid, int64_t *counts, void *stream);
 
 /* ------------------------------------------------------------------------
+ * Sequence operators on channels-last activations, the inference forms.  They
+ * stand beside the models' own stages for frame classifiers that normalise
+ * without batch statistics and mix frames with a linear recurrence; the
+ * reference has none of them (its models use BatchNorm, nnet/CNN.py:66-98, and
+ * GRUs, nnet/RNN.py:19-30, models.py:114).
+ *
+ * Activations are float32, float16 or bfloat16 (SEDMI_DTYPE_*), one type per
+ * call; parameters (weights, biases, A, D) and scan states are float32, sums,
+ * statistics and states are held in float32, results are rounded once.  Rows
+ * may start at any address that is a multiple of the element size.
+ * lengths: device int64 [n_clips] or NULL (= all frames).  Frames at and behind
+ * lengths[i] (clamped to 0 .. frames) are never read, and their outputs are 0.
+ * ------------------------------------------------------------------------ */
+#define SEDMI_DTYPE_F32   0
+#define SEDMI_DTYPE_F16   1
+#define SEDMI_DTYPE_BF16  2
+
+#define SEDMI_ACT_NONE    0
+#define SEDMI_ACT_RELU    1
+#define SEDMI_ACT_SILU    2   /* x * sigmoid(x) */
+#define SEDMI_ACT_GELU    3   /* x * (1 + erf(x / sqrt 2)) / 2 */
+
+/* y = act((x - mean) / sqrt(var + eps) * weight[c] + bias[c]) with mean and
+ * biased variance over the valid frames, all inner positions and the
+ * channels / groups channels of a clip's group.
+ *   x, y         device [n_clips, frames, inner, channels], contiguous; y may be x
+ *   weight, bias device float32 [channels] or NULL (1 and 0)
+ *   ws           device scratch >= sedmi_group_norm_workspace_bytes() */
+size_t sedmi_group_norm_workspace_bytes(int64_t n_clips, int64_t frames, int64_t inner, int channels, int groups,
+                                        int dtype);
+int sedmi_group_norm(const void *x, const float *weight, const float *bias, const int64_t *lengths, void *y,
+                     int64_t n_clips, int64_t frames, int64_t inner, int channels, int groups, float eps,
+                     int activation, int dtype, void *ws, size_t ws_bytes, void *stream);
+
+/* Depthwise convolution over time that looks at the current and the width - 1
+ * earlier frames:
+ *   y[i, t, c] = act(bias[c] + sum_k weight[c, k] * x[i, t - (width - 1) + k, c])
+ *   x          device [n_clips, frames, channels], channels adjacent, the other
+ *              two strides given in elements
+ *   weight     device float32 [channels, width], 1 <= width <= 8; bias float32 [channels] or NULL
+ *   state_in   device [n_clips, width - 1, channels] of the type of x: the inputs before the first
+ *              frame, oldest first; NULL = zeros
+ *   state_out  the same shape: the last width - 1 inputs (state and valid frames); NULL = not wanted;
+ *              may be state_in itself, must not overlap it otherwise.  A call with frames = 1 and
+ *              state_out == state_in is the form for one new frame per stream.
+ *   reverse    nonzero: runs from the last valid frame to the first (the state then holds what comes
+ *              behind the last frame)
+ *   y          device [n_clips, frames, channels], contiguous; must not overlap x or the states */
+int sedmi_causal_conv1d(const void *x, int64_t x_stride_clip, int64_t x_stride_frame, const float *weight,
+                        const float *bias, const int64_t *lengths, const void *state_in, void *state_out, void *y,
+                        int64_t n_clips, int64_t frames, int channels, int width, int activation, int reverse,
+                        int dtype, void *stream);
+
+/* Selective state space scan:
+ *   d = dt + dt_bias, or softplus(dt + dt_bias) with dt_softplus
+ *   h[c, n] <- exp(d[c] A[c, n]) h[c, n] + d[c] x[c] B[g(c), n]
+ *   y[c] = (sum_n C[g(c), n] h[c, n] + D[c] x[c]) * silu(z[c])
+ * frame after frame, g(c) = c / (channels / groups).  In x, dt, z, B and C the
+ * last dimension is contiguous and the others have strides in elements; y, A, D,
+ * dt_bias and the states are contiguous.  y and state_out overlap none of the inputs. */
+typedef struct sedmi_scan_args {
+    const void *x, *dt, *z;                 /* [n_clips, frames, channels]; z NULL = no gate              */
+    const void *B, *C;                      /* [n_clips, frames, groups, states]                          */
+    const float *A, *D, *dt_bias;           /* [channels, states], [channels] or NULL, [channels] or NULL */
+    const int64_t *lengths;                 /* [n_clips] or NULL                                          */
+    const float *state_in;                  /* [n_clips, channels, states], NULL = zeros                  */
+    float *state_out;                       /* the same, NULL = not wanted                                */
+    void *y;                                /* [n_clips, frames, channels]                                */
+    int64_t x_stride[2], dt_stride[2], z_stride[2];        /* clip, frame                                 */
+    int64_t B_stride[3], C_stride[3];                      /* clip, frame, group                          */
+    int64_t n_clips, frames;
+    int channels, groups, states;           /* states: 1 .. 128                                           */
+    int dtype, dt_softplus, reverse;        /* reverse: from the last valid frame to the first            */
+} sedmi_scan_args;
+
+size_t sedmi_selective_scan_workspace_bytes(int64_t n_clips, int64_t frames, int channels, int groups, int states);
+int sedmi_selective_scan(const sedmi_scan_args *args, void *ws, size_t ws_bytes, void *stream);
+/* The form for one new frame per stream: frames = 1, no lengths, not reversed, and the state is updated in place
+ * (state_in == state_out). */
+int sedmi_selective_step(const sedmi_scan_args *args, void *stream);
+
+/* ------------------------------------------------------------------------
  * Per-kernel timing (no counterpart in the reference; it exists so that a
  * benchmark can quote each kernel's duration and its algorithmic FLOP / byte
  * rate from HIP events recorded on the very stream the kernels run on).

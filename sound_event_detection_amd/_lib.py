@@ -82,6 +82,19 @@ class BasicRcnnWeights(C.Structure):
                 ("gru_w_ih", _FP), ("gru_w_hh", _FP), ("gru_b_ih", _FP), ("gru_b_hh", _FP), ("fc_w", _FP), ("fc_b", _FP)]
 
 
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3
+
+
+class ScanArgs(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("x", "dt", "z", "B", "C", "A", "D", "dt_bias", "lengths", "state_in",
+                                           "state_out", "y")]
+                + [(n, C.c_int64 * 2) for n in ("x_stride", "dt_stride", "z_stride")]
+                + [(n, C.c_int64 * 3) for n in ("B_stride", "C_stride")]
+                + [(n, C.c_int64) for n in ("n_clips", "frames")]
+                + [(n, C.c_int) for n in ("channels", "groups", "states", "dtype", "dt_softplus", "reverse")])
+
+
 class KernelStat(C.Structure):
     _fields_ = [("name", C.c_char * 48), ("launches", C.c_int64), ("ms", C.c_double),
                 ("flops", C.c_double), ("bytes", C.c_double)]
@@ -132,6 +145,12 @@ SIGNATURES = {
     "sedmi_decode_events_static": (_I, [_VP, _I64, _I, _VP, _VP, _I64, _F, _I, _I, _VP, _VP, _VP, _VP,
                                         _I64, _VP, _VP]),
     "sedmi_confusion_counts": (_I, [_VP, _VP, _I64, _I, _F, _I, _VP, _VP]),
+    "sedmi_group_norm_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I, _I, _I]),
+    "sedmi_group_norm": (_I, [_VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _I, _I, _F, _I, _I, _VP, _SZ, _VP]),
+    "sedmi_causal_conv1d": (_I, [_VP, _I64, _I64, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I, _I, _I, _I, _I, _VP]),
+    "sedmi_selective_scan_workspace_bytes": (_SZ, [_I64, _I64, _I, _I, _I]),
+    "sedmi_selective_scan": (_I, [C.POINTER(ScanArgs), _VP, _SZ, _VP]),
+    "sedmi_selective_step": (_I, [C.POINTER(ScanArgs), _VP]),
     "sedmi_profile_enable": (_I, [_I]),
     "sedmi_profile_collect": (_I, [C.POINTER(KernelStat), _I]),
 }
