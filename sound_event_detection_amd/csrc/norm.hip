@@ -8,6 +8,7 @@
 #include "common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 #include "vec_io.h"
@@ -60,7 +61,7 @@ __global__ __launch_bounds__(kThreads) void norm_stats_kernel(const T *x, NormAr
                 const float inv = __builtin_amdgcn_rcpf(n);
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    const float v = static_cast<float>(p.v[e]), d = v - mean[e];
+                    const float v = p.get(e), d = v - mean[e];
                     mean[e] = fmaf(d, inv, mean[e]);
                     m2[e] = fmaf(d, v - mean[e], m2[e]);
                 }
@@ -171,15 +172,13 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(const T *x, T *y, 
         }
         for (int64_t r = r0 + row; r < r1; r += rp) {
             const int64_t at = at0 + r * a.channels + j * V;
-            Pack<T, V> out;
+            Pack<T, V> out = Pack<T, V>::zero();
             if (r < valid) {
                 const auto p = load_pack<T, V>(x + at, ne);
+                float v[V];
 #pragma unroll
-                for (int e = 0; e < V; ++e)
-                    out.v[e] = static_cast<T>(activate(fmaf(static_cast<float>(p.v[e]) - mean[e], scale[e], shift[e]), a.act));
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; ++e) out.v[e] = static_cast<T>(0.0f);
+                for (int e = 0; e < V; ++e) v[e] = activate(fmaf(p.get(e) - mean[e], scale[e], shift[e]), a.act);
+                out = Pack<T, V>::from(v);
             }
             store_pack<T, V>(y + at, out, ne);
         }

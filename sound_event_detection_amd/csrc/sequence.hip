@@ -3,6 +3,7 @@
 #include "common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 #include "vec_io.h"
@@ -42,79 +43,87 @@ __global__ __launch_bounds__(kThreads) void causal_conv_kernel(const T *x, const
     const int64_t sx = a.reverse ? -a.x_frame : a.x_frame, sy = a.reverse ? -a.channels : a.channels;
     const int64_t state_at = clip * H * a.channels + c0;
 
-    float w[V][K], b[V];
+    // the V x K weights of these channels are adjacent
+    Pack<float, 4> wp[V * K / 4], bp[V / 4];
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-        const int c = min(c0 + e, a.channels - 1);
+    for (int i = 0; i < V * K / 4; ++i)
+        wp[i] = load_pack<float, 4>(a.weight + static_cast<int64_t>(c0) * K + min(4 * i, ne * K - 1), ne * K - 4 * i);
 #pragma unroll
-        for (int k = 0; k < K; ++k) w[e][k] = a.weight[static_cast<int64_t>(c) * K + k];
-        b[e] = a.bias ? a.bias[c] : 0.0f;
-    }
-    const int64_t t0 = static_cast<int64_t>(segment) * a.rows, t1 = min(t0 + a.rows, a.frames);
-    float past[H > 0 ? H : 1][V];
-    Pack<T, V> old[H > 0 ? H : 1];                               // the state: only the first run of a clip looks at it
-#pragma unroll
-    for (int i = 0; i < H; ++i) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) old[i].v[e] = static_cast<T>(0.0f);
-        if (segment == 0 && state_in != nullptr)
-            old[i] = load_pack<T, V>(state_in + state_at + static_cast<int64_t>(i) * a.channels, ne);
-    }
+    for (int i = 0; i < V / 4; ++i)
+        bp[i] = a.bias ? load_pack<float, 4>(a.bias + c0 + min(4 * i, ne - 1), ne - 4 * i) : Pack<float, 4>::zero();
+    auto w = [&](int e, int k) { return wp[(e * K + k) / 4].get((e * K + k) % 4); };
+    const int64_t t0 = static_cast<int64_t>(segment) * a.rows, t1 = min(t0 + a.rows, a.frames), tv = min(t1, length);
+    Pack<T, V> win[H + U];                                       // the inputs as they are: H past ones, then U new ones
 #pragma unroll
     for (int i = 0; i < H; ++i) {
         const int64_t t = t0 - H + i;                            // rows >= H: a later run never reaches the state
-        Pack<T, V> p = old[i];
-        if (t >= 0 && t < length) p = load_pack<T, V>(px + t * sx, ne);
-#pragma unroll
-        for (int e = 0; e < V; ++e) past[i][e] = static_cast<float>(p.v[e]);
+        if (t >= 0 && t < length) {
+            win[i] = load_pack<T, V>(px + t * sx, ne);
+        } else if (t < 0 && state_in != nullptr) {
+            win[i] = load_pack<T, V>(state_in + state_at + static_cast<int64_t>(i) * a.channels, ne);
+        } else {
+            win[i] = Pack<T, V>::zero();
+        }
     }
     if (segment == 0 && state_out != nullptr) {
-        // the last H inputs of (state, valid frames), oldest first; read before written, so state_out may be state_in
+        // the last H inputs of (state, valid frames), oldest first; this lane alone looks at its channels of the state
+        // and has read them, so state_out may be state_in
+        Pack<T, V> last[H > 0 ? H : 1];
 #pragma unroll
         for (int i = 0; i < H; ++i) {
             const int64_t t = length - H + i;
-            Pack<T, V> p;
             if (t >= 0) {
-                p = load_pack<T, V>(px + t * sx, ne);
+                last[i] = load_pack<T, V>(px + t * sx, ne);
             } else {
-                p = old[0];
+                last[i] = win[0];
 #pragma unroll
                 for (int k = 1; k < H; ++k)
-                    if (t + H == k) p = old[k];
+                    if (t + H == k) last[i] = win[k];
             }
-            store_pack<T, V>(state_out + state_at + static_cast<int64_t>(i) * a.channels, p, ne);
         }
+#pragma unroll
+        for (int i = 0; i < H; ++i)
+            store_pack<T, V>(state_out + state_at + static_cast<int64_t>(i) * a.channels, last[i], ne);
     }
-    for (int64_t t = t0; t < t1; t += U) {
-        Pack<T, V> in[U];
+    auto fetch = [&](int64_t t, Pack<T, V> *to) {                // frames behind the end repeat the last one
+#pragma unroll
+        for (int u = 0; u < U; ++u) to[u] = load_pack<T, V>(px + min(t + u, tv - 1) * sx, ne);
+    };
+    Pack<T, V> next[U];
+    if (t0 < tv) fetch(t0, next);
+    for (int64_t t = t0; t < tv; t += U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) win[H + u] = next[u];
+        if (t + U < tv) fetch(t + U, next);
+        Pack<T, V> out[U];
+        constexpr int P = Pack<T, V>::kPer;
+#pragma unroll
+        for (int i = 0; i < V / P; ++i) {                        // a word of channels at a time
+            float s[U][P];
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                float f[H + U];
+#pragma unroll
+                for (int r = 0; r < H + U; ++r) f[r] = win[r].get(i * P + e);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    float v = bp[(i * P + e) / 4].get((i * P + e) % 4);
+#pragma unroll
+                    for (int k = 0; k < K; ++k) v = fmaf(w(i * P + e, k), f[u + k], v);
+                    s[u][e] = activate(v, a.act);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) out[u].set_word(i, s[u]);
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (t + u < min(t1, length)) in[u] = load_pack<T, V>(px + (t + u) * sx, ne);
+            if (t + u < tv) store_pack<T, V>(py + (t + u) * sy, out[u], ne);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (t + u >= t1) break;
-            Pack<T, V> out;
-            if (t + u < length) {
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float v = static_cast<float>(in[u].v[e]);
-                    float s = b[e];
-#pragma unroll
-                    for (int k = 0; k < H; ++k) s = fmaf(w[e][k], past[k][e], s);
-                    s = fmaf(w[e][H], v, s);
-#pragma unroll
-                    for (int k = 0; k + 1 < H; ++k) past[k][e] = past[k + 1][e];
-                    if (H > 0) past[H > 0 ? H - 1 : 0][e] = v;
-                    out.v[e] = static_cast<T>(activate(s, a.act));
-                }
-                store_pack<T, V>(py + (t + u) * sy, out, ne);
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; ++e) out.v[e] = static_cast<T>(0.0f);
-                store_pack<T, V>(y + (clip * a.frames + t + u) * a.channels + c0, out, ne);
-            }
-        }
+        for (int i = 0; i < H; ++i) win[i] = win[U + i];
     }
+    for (int64_t t = max(t0, length); t < t1; ++t)
+        store_pack<T, V>(y + (clip * a.frames + t) * a.channels + c0, Pack<T, V>::zero(), ne);
 }
 
 constexpr int kMaxWidth = 8;
@@ -150,7 +159,7 @@ int launch_conv(int width, unsigned blocks, hipStream_t st, const void *x, const
 // once per (frame, channel) instead of once per lane, and the four lanes of a channel read them as broadcasts.
 constexpr int kChannels = 64;            // per workgroup
 constexpr int kTile = 32;                // frames staged at a time
-constexpr int kYStride = kChannels + 16; // the four rows a quad group writes land in different banks
+constexpr int kYStride = kChannels + 16; // of the y tile: rows a wave writes together lie in different banks
 
 struct ScanArgs {
     const void *x, *dt, *B, *C, *z;
@@ -171,27 +180,24 @@ struct ScanArgs {
     float *end_step;                     // [clips][splits - 1][channels]: sum of its step sizes
 };
 
-// log(1 + exp(x)) = max(x, 0) + log1p(e), e = exp(-|x|) <= 1, and log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3, by its
-// series: s^2 <= 1/9, the terms left out are below 2^-26 of the sum.  Step sizes of 1e-3 keep all their bits.
+// log(1 + exp(x)) = max(x, 0) + log1p(e), e = exp(-|x|) <= 1, and log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3:
+// atanh(s) = s + s q P(q), q = s^2 <= 1/9, with P the polynomial of degree 3 that is nearest to the series
+// 1/3 + q/5 + q^2/7 + ... there (4.5e-9 of the result).  Step sizes of 1e-3 keep all their bits, which a logarithm of
+// the rounded sum 1 + e would not give them.
 __device__ __forceinline__ float softplus(float x) {
     const float e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(x));
-    const float s = e / (2.0f + e), q = s * s;
-    float p = 1.0f / 15.0f;
-    p = fmaf(p, q, 1.0f / 13.0f);
-    p = fmaf(p, q, 1.0f / 11.0f);
-    p = fmaf(p, q, 1.0f / 9.0f);
-    p = fmaf(p, q, 1.0f / 7.0f);
-    p = fmaf(p, q, 1.0f / 5.0f);
-    p = fmaf(p, q, 1.0f / 3.0f);
-    const float log1p = 2.0f * fmaf(p * q, s, s);
-    return x != x ? x : fmaxf(x, 0.0f) + log1p;
+    const float s = e * __builtin_amdgcn_rcpf(2.0f + e), q = s * s;
+    float p = fmaf(0.14005976f, q, 0.14000906f);
+    p = fmaf(p, q, 0.20010763f);
+    p = fmaf(p, q, 0.33333208f);
+    const float half = fmaf(p * q, s, s);
+    return fmaf(2.0f, half, fmaxf(x, 0.0f));             // a NaN comes through e
 }
 
-// Sum over the four lanes of a quad (DPP quad_perm: no LDS).
-__device__ __forceinline__ float quad_sum(float v) {
-    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true));
-    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true));
-    return v;
+// Value of the lane n before this one in its row of 16 (DPP rotation: no LDS).
+template <int N>
+__device__ __forceinline__ float from_lane_before(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + N, 0xF, 0xF, true));
 }
 
 // A * log2(e), so that exp(d A) is one exp2 of a product; -inf is taken as the lowest finite number, for which a step
@@ -201,13 +207,34 @@ __device__ __forceinline__ float decay_rate(float a) {
     return r < -3.402823466e38f ? -3.402823466e38f : r;
 }
 
+// The element behind the first of a pair, moved to its place.
+template <typename T>
+__device__ __forceinline__ Pack<T, 2> second_first(Pack<T, 2> p, bool move) {
+    if constexpr (sizeof(T) == 2) p.w[0] >>= move ? 16 : 0;
+    else p.w[0] = move ? p.w[1] : p.w[0];
+    return p;
+}
+
+using F4 = __attribute__((ext_vector_type(4))) float;
+
+// Lane v of a wave holds channel (v & 3) + 4 (v >> 4) of the wave's 16 and quarter q = (v >> 2) & 3 of its states: with
+// NP >= 4 states per lane those are n = 16 k + 4 q + i, k < NP / 4, i < 4.  That is the layout of sixteen 4 x 4 blocks of
+// the matrix instruction v_mfma_f32_4x4x1 (row i in register i, column = lane & 3), so d x B^T, an outer product of 4
+// channels and 4 states per block, is added to exp(d A) h by the matrix unit while the vector unit, which bounds this
+// kernel, forms the next exponents.  Up to 8 states (NP < 4) a lane holds n = q NP + i and adds them itself.
+//
+// Two workgroups per compute unit at least: with at most 256 registers the compiler keeps the matrix instruction's
+// accumulators in ordinary registers, which saves eight moves per frame.
 template <typename T, int NP, bool END>
-__global__ __launch_bounds__(kThreads) void selective_scan_kernel(ScanArgs a) {
+__global__ __launch_bounds__(kThreads, 2) void selective_scan_kernel(ScanArgs a) {
     constexpr int N4 = 4 * NP;                                   // states staged per frame, zero beyond a.states
-    constexpr int kB = (kTile * N4 + kThreads - 1) / kThreads;   // of them per thread
+    constexpr bool kMatrix = NP >= 4;
+    constexpr int kBRows = kThreads / N4 < kTile ? kThreads / N4 : kTile;    // rows of B that the workgroup loads at a time
+    constexpr int kB = kTile / kBRows;
+    constexpr int kJoin = NP <= 8 ? 8 : 2;                       // runs whose ends are in flight together
     __shared__ float s_step[kTile][kChannels][2];                // d, d * x
     __shared__ __attribute__((aligned(16))) float s_b[kTile][N4], s_c[END ? 1 : kTile][N4];
-    __shared__ float s_y[END ? 1 : kTile][kYStride];
+    __shared__ float s_y[END ? 1 : kTile + 2][kYStride];         // the last two rows: what half of the lanes need not write
 
     const int tid = threadIdx.x;
     unsigned rest = blockIdx.x;
@@ -222,159 +249,255 @@ __global__ __launch_bounds__(kThreads) void selective_scan_kernel(ScanArgs a) {
     const int width = min(kChannels, a.per_group - first);
     const int64_t length = clamp_length(a.lengths, clip, a.frames);
     const int64_t t0 = split * a.run;
-    const int64_t t1 = min(t0 + a.run, length);                  // may lie before t0: nothing to do
+    const int64_t count = min(t0 + a.run, length) - t0;          // valid frames of this run, <= 0: none
 
+    // staging: two channels of one row per lane, four rows 8 apart per thread.  Of an odd number of channels the last
+    // lane loads the pair before it and takes the second; lanes beside the last channel load the last pair for nothing.
     const int64_t turn = a.reverse && length > 0 ? length - 1 : 0;
     const int dir = a.reverse ? -1 : 1;
-    // staging: two channels of one row per lane, four rows 8 apart per thread
     const int sc = (tid & 31) * 2, sr = tid >> 5;
-    const int sn = min(2, width - sc);
-    const T *px = static_cast<const T *>(a.x) + clip * a.x_clip + turn * a.x_frame + c0 + sc;
-    const T *pd = static_cast<const T *>(a.dt) + clip * a.dt_clip + turn * a.dt_frame + c0 + sc;
-    const T *pz = a.z ? static_cast<const T *>(a.z) + clip * a.z_clip + turn * a.z_frame + c0 + sc : nullptr;
-    const T *pb = static_cast<const T *>(a.B) + clip * a.b_clip + turn * a.b_frame + group * a.b_group;
-    const T *pc = static_cast<const T *>(a.C) + clip * a.c_clip + turn * a.c_frame + group * a.c_group;
-    T *py = static_cast<T *>(a.y) + clip * a.frames * a.channels + c0 + sc;
+    const int sn = min(2, width - sc), pair = max(0, min(sc, width - 2));
+    const bool second = sc - pair == 1 && width > 1;
+    const int64_t row0 = turn + dir * t0;
+    const int64_t sx = dir * a.x_frame, sd = dir * a.dt_frame, sz = dir * a.z_frame;
+    const int64_t sb = dir * a.b_frame, sv = dir * a.c_frame, sy = dir * a.channels;
+    const T *px = static_cast<const T *>(a.x) + clip * a.x_clip + row0 * a.x_frame + c0;
+    const T *pd = static_cast<const T *>(a.dt) + clip * a.dt_clip + row0 * a.dt_frame + c0;
+    const T *pz = static_cast<const T *>(a.z) + (a.z ? clip * a.z_clip + row0 * a.z_frame + c0 : 0);
+    const T *pb = static_cast<const T *>(a.B) + clip * a.b_clip + row0 * a.b_frame + group * a.b_group;
+    const T *pc = static_cast<const T *>(a.C) + clip * a.c_clip + row0 * a.c_frame + group * a.c_group;
+    T *py = static_cast<T *>(a.y) + (clip * a.frames + row0) * a.channels + c0;
+    const int64_t ox = sr * sx + pair, od = sr * sd + pair, oz = sr * sz + pair, oy = sr * sy + sc;
+    const int br = min(tid / N4, kTile - 1), bn = tid % N4, bl = min(bn, a.states - 1);
+    const int64_t ob = br * sb + bl, oc = br * sv + bl;
+    const bool gate = !END && a.z != nullptr;
     float bias[2], skip[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-        bias[e] = a.dt_bias && e < sn ? a.dt_bias[c0 + sc + e] : 0.0f;
-        skip[e] = !END && a.D && e < sn ? a.D[c0 + sc + e] : 0.0f;
+        const int c = c0 + min(sc + e, width - 1);
+        bias[e] = a.dt_bias ? a.dt_bias[c] : 0.0f;
+        skip[e] = !END && a.D ? a.D[c] : 0.0f;
     }
 
-    // compute: channel ch of the workgroup, states q * NP ...
-    const int ch = tid >> 2, q = tid & 3;
+    // compute: a lane past the last channel repeats it, a state past the last has rate, input and output zero
+    const int lane = tid & 63, q = (lane >> 2) & 3;
+    const int ch = (tid >> 6) * 16 + (lane >> 4) * 4 + (lane & 3);
     const bool live = ch < width;
+    const int cl = c0 + min(ch, width - 1);
+    auto state_of = [&](int j) __attribute__((always_inline)) { return kMatrix ? 16 * (j / 4) + 4 * q + j % 4 : q * NP + j; };
     float rate[NP], h[NP], total = 0.0f;
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-        const int n = q * NP + j;
-        rate[j] = live && n < a.states ? decay_rate(a.A[static_cast<int64_t>(c0 + ch) * a.states + n]) : 0.0f;
+        const int n = state_of(j);
+        const float v = a.A[static_cast<int64_t>(cl) * a.states + min(n, a.states - 1)];
+        rate[j] = n < a.states ? decay_rate(v) : 0.0f;
         h[j] = 0.0f;
     }
     if (!END) {
         if (a.state_in != nullptr) {
 #pragma unroll
             for (int j = 0; j < NP; ++j) {
-                const int n = q * NP + j;
-                if (live && n < a.states) h[j] = a.state_in[(clip * a.channels + c0 + ch) * a.states + n];
+                const int n = state_of(j);
+                const float v = a.state_in[(clip * a.channels + cl) * a.states + min(n, a.states - 1)];
+                h[j] = n < a.states ? v : 0.0f;
             }
         }
-        for (int s = 0; s < split; ++s) {                        // the runs before this one, joined
-            const int64_t at = (clip * (a.splits - 1) + s) * a.channels + c0 + ch;
-            const float d = live ? a.end_step[at] : 0.0f;
+        for (int s = 0; s < split; s += kJoin) {                 // the runs before this one, joined
+            float d[kJoin], e[kJoin][NP];
 #pragma unroll
-            for (int j = 0; j < NP; ++j) {
-                const int n = q * NP + j;
-                const float e = live && n < a.states ? a.end_state[at * a.states + n] : 0.0f;
-                h[j] = fmaf(__builtin_amdgcn_exp2f(d * rate[j]), h[j], e);
+            for (int k = 0; k < kJoin; ++k) {
+                const int64_t at = (clip * (a.splits - 1) + min(s + k, split - 1)) * a.channels + cl;
+                d[k] = a.end_step[at];
+#pragma unroll
+                for (int j = 0; j < NP; ++j) e[k][j] = a.end_state[at * a.states + min(state_of(j), a.states - 1)];
+            }
+#pragma unroll
+            for (int k = 0; k < kJoin; ++k) {
+                if (s + k >= split) break;
+#pragma unroll
+                for (int j = 0; j < NP; ++j)
+                    h[j] = fmaf(__builtin_amdgcn_exp2f(d[k] * rate[j]), h[j], state_of(j) < a.states ? e[k][j] : 0.0f);
             }
         }
     }
 
-    Pack<T, 2> rx[4], rd[4], rz[4];
-    float rb[kB], rc[kB];
-    auto fetch = [&](int64_t t) {
+    Pack<T, 2> rx[4], rd[4], rz[4] = {};
+    T rb[kB], rc[kB];
+    // The next rows of the run, `left` of them valid; rows past them repeat the last.  kWhole: all kTile are valid;
+    // kRows: fewer; kOne: the block has one channel, beside which there may be no memory.
+    enum { kWhole, kRows, kOne };
+    auto load = [&](auto mode, const T *p, int i, int64_t stride, int64_t at, int left) __attribute__((always_inline)) {
+        if constexpr (decltype(mode)::value == kWhole) {
+            return load_pack<T, 2>(p + 8 * i * stride + at, 2);
+        } else {
+            const T *row = p + min(sr + 8 * i, left - 1) * stride;
+            if constexpr (decltype(mode)::value == kRows) return load_pack<T, 2>(row + pair, 2);
+            else return load_pack<T, 2>(row, 1);
+        }
+    };
+    auto fetch = [&](auto mode, int left) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t r = t + sr + 8 * i;
-            const int n = r < t1 ? sn : 0;
-            rx[i] = load_pack<T, 2>(px + dir * r * a.x_frame, n);
-            rd[i] = load_pack<T, 2>(pd + dir * r * a.dt_frame, n);
-            if (!END && pz) rz[i] = load_pack<T, 2>(pz + dir * r * a.z_frame, n);
+        for (int i = 0; i < 4; ++i) rx[i] = load(mode, px, i, sx, ox, left), rd[i] = load(mode, pd, i, sd, od, left);
+        if (gate) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) rz[i] = load(mode, pz, i, sz, oz, left);
+            pz += kTile * sz;
         }
 #pragma unroll
         for (int i = 0; i < kB; ++i) {
-            const int at = tid + i * kThreads, r = at / N4, n = at % N4;
-            const bool on = r < kTile && t + r < t1 && n < a.states;
-            rb[i] = on ? static_cast<float>(pb[dir * (t + r) * a.b_frame + n]) : 0.0f;
-            if (!END) rc[i] = on ? static_cast<float>(pc[dir * (t + r) * a.c_frame + n]) : 0.0f;
+            if constexpr (decltype(mode)::value == kWhole) {
+                rb[i] = pb[i * kBRows * sb + ob];
+                if (!END) rc[i] = pc[i * kBRows * sv + oc];
+            } else {
+                const int r = min(br + i * kBRows, left - 1);
+                rb[i] = pb[r * sb + bl];
+                if (!END) rc[i] = pc[r * sv + bl];
+            }
         }
+        px += kTile * sx, pd += kTile * sd, pb += kTile * sb, pc += kTile * sv;
     };
-    if (t0 < t1) fetch(t0);
-    for (int64_t t = t0; t < t1; t += kTile) {
-        Pack<T, 2> cx[4], cz[4];
+    auto fetch_any = [&](int left) __attribute__((always_inline)) {
+        if (left == kTile && width > 1) fetch(std::integral_constant<int, kWhole>{}, kTile);
+        else if (width > 1) fetch(std::integral_constant<int, kRows>{}, left);
+        else fetch(std::integral_constant<int, kOne>{}, left);
+    };
+    auto stage = [&](auto whole, auto soft, int left) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int r = sr + 8 * i;
+            rd[i] = second_first(rd[i], second), rx[i] = second_first(rx[i], second);
             float step[2], in[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float v = static_cast<float>(rd[i].v[e]) + bias[e];
-                const bool on = t + r < t1 && e < sn;            // behind the end: a step of zero keeps the state
-                step[e] = on ? (a.softplus ? softplus(v) : v) : 0.0f;
-                in[e] = on ? step[e] * static_cast<float>(rx[i].v[e]) : 0.0f;
+                const float v = rd[i].get(e) + bias[e];
+                step[e] = decltype(soft)::value ? softplus(v) : v;
+                in[e] = step[e] * rx[i].get(e);
+                if (!decltype(whole)::value && r >= left) step[e] = in[e] = 0.0f;    // a step of zero keeps the state
             }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) s_step[r][sc + e][0] = step[e], s_step[r][sc + e][1] = in[e];
-            cx[i] = rx[i];
-            if (!END) cz[i] = rz[i];
+            *reinterpret_cast<F4 *>(&s_step[r][sc][0]) = F4{step[0], in[0], step[1], in[1]};
         }
 #pragma unroll
         for (int i = 0; i < kB; ++i) {
-            const int at = tid + i * kThreads;
-            if (kTile * N4 >= kThreads || at < kTile * N4) {
-                s_b[at / N4][at % N4] = rb[i];
-                if (!END) s_c[at / N4][at % N4] = rc[i];
+            const int r = br + i * kBRows;
+            const bool on = bn < a.states && (decltype(whole)::value || r < left);
+            if (kB > 1 || tid / N4 < kTile) {
+                s_b[r][bn] = on ? static_cast<float>(rb[i]) : 0.0f;
+                if (!END) s_c[r][bn] = on ? static_cast<float>(rc[i]) : 0.0f;
             }
         }
+    };
+    // sums of y over the quarters for four frames: the lanes 8 apart exchange halves, then those of the odd quarters add
+    // their neighbours' and have two frames each
+    const bool high = q & 2;
+    float *const y_base = &s_y[END ? 0 : (q & 1 ? q - 1 : kTile)][ch];
+    const int y_step = q & 1 ? 4 * kYStride : 0;
+
+    auto left_at = [&](int64_t t) __attribute__((always_inline)) { return static_cast<int>(min(static_cast<int64_t>(kTile), count - t)); };
+    if (count > 0) fetch_any(left_at(0));
+    for (int64_t t = 0; t < count; t += kTile) {
+        const int left = left_at(t);
+        const bool whole = left == kTile;
+        Pack<T, 2> cx[4], cz[4];
+        if (whole && a.softplus) stage(std::true_type{}, std::true_type{}, kTile);
+        else if (a.softplus) stage(std::false_type{}, std::true_type{}, left);
+        else stage(std::false_type{}, std::false_type{}, left);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) cx[i] = rx[i], cz[i] = second_first(rz[i], second);
         __syncthreads();
-        if (t + kTile < t1) fetch(t + kTile);
-        const int steps = static_cast<int>(min(static_cast<int64_t>(kTile), t1 - t));
-        for (int r = 0; r < steps; r += 4) {
+        if (t + kTile < count) fetch_any(left_at(t + kTile));
+        float *y_at = y_base;
+        for (int r = 0; r < left; r += 4) {
             float out[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const float d = s_step[r + u][ch][0], v = s_step[r + u][ch][1];
                 float y = 0.0f;
+                if constexpr (kMatrix) {
 #pragma unroll
-                for (int j = 0; j < NP; ++j) {
-                    h[j] = fmaf(__builtin_amdgcn_exp2f(d * rate[j]), h[j], v * s_b[r + u][q * NP + j]);
-                    if (!END) y = fmaf(h[j], s_c[r + u][q * NP + j], y);
+                    for (int k = 0; k < NP / 4; ++k) {
+                        F4 next;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) next[i] = __builtin_amdgcn_exp2f(d * rate[4 * k + i]) * h[4 * k + i];
+                        next = __builtin_amdgcn_mfma_f32_4x4x1f32(s_b[r + u][16 * k + 4 * q + (lane & 3)], v, next, 0, 0, 0);
+                        F4 c;
+                        if (!END) c = *reinterpret_cast<const F4 *>(&s_c[r + u][16 * k + 4 * q]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            h[4 * k + i] = next[i];
+                            if (!END) y = fmaf(next[i], c[i], y);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < NP; ++j) {
+                        h[j] = fmaf(__builtin_amdgcn_exp2f(d * rate[j]), h[j], v * s_b[r + u][q * NP + j]);
+                        if (!END) y = fmaf(h[j], s_c[r + u][q * NP + j], y);
+                    }
                 }
                 if (END) total += d;
-                else out[u] = quad_sum(y);
+                else out[u] = y;
             }
-            if (!END) s_y[r + q][ch] = q == 0 ? out[0] : q == 1 ? out[1] : q == 2 ? out[2] : out[3];
+            if (!END) {
+                float k0 = high ? out[2] : out[0], k1 = high ? out[3] : out[1];
+                k0 += from_lane_before<8>(high ? out[0] : out[2]);
+                k1 += from_lane_before<8>(high ? out[1] : out[3]);
+                y_at[0] = k0 + from_lane_before<4>(k0);
+                y_at[kYStride] = k1 + from_lane_before<4>(k1);
+                y_at += y_step;
+            }
         }
         __syncthreads();
         if (!END) {
+            auto write = [&](auto all, auto gated) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = sr + 8 * i;
-                if (t + r >= t1 || sn <= 0) continue;
-                Pack<T, 2> out;
+                for (int i = 0; i < 4; ++i) {
+                    const int r = sr + 8 * i;
+                    float v[2];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float v = fmaf(skip[e], static_cast<float>(cx[i].v[e]), s_y[r][sc + e]);
-                    if (pz) v *= silu(static_cast<float>(cz[i].v[e]));
-                    out.v[e] = static_cast<T>(v);
+                    for (int e = 0; e < 2; ++e) {
+                        v[e] = fmaf(skip[e], cx[i].get(e), s_y[r][sc + e]);
+                        if (decltype(gated)::value) v[e] *= silu(cz[i].get(e));
+                    }
+                    T *to = py + 8 * i * sy + oy;
+                    if constexpr (decltype(all)::value) store_pack<T, 2>(to, Pack<T, 2>::from(v), 2);
+                    else if (r < left && sn > 0) store_pack<T, 2>(to, Pack<T, 2>::from(v), sn);
                 }
-                store_pack<T, 2>(py + (turn + dir * (t + r)) * a.channels, out, sn);
-            }
+                py += kTile * sy;
+            };
+            const bool all = whole && width == kChannels;
+            if (all && gate) write(std::true_type{}, std::true_type{});
+            else if (all) write(std::true_type{}, std::false_type{});
+            else if (gate) write(std::false_type{}, std::true_type{});
+            else write(std::false_type{}, std::false_type{});
         }
     }
     if (END) {
-        const int64_t at = (clip * (a.splits - 1) + split) * a.channels + c0 + ch;
+        const int64_t at = (clip * (a.splits - 1) + split) * a.channels + cl;
         if (live) {
             if (q == 0) a.end_step[at] = total;
 #pragma unroll
             for (int j = 0; j < NP; ++j)
-                if (q * NP + j < a.states) a.end_state[at * a.states + q * NP + j] = h[j];
+                if (state_of(j) < a.states) a.end_state[at * a.states + state_of(j)] = h[j];
         }
         return;
     }
     if (sn > 0) {                                                // frames behind the clip's end
-        Pack<T, 2> zero;
-        zero.v[0] = zero.v[1] = static_cast<T>(0.0f);
+        T *pe = static_cast<T *>(a.y) + clip * a.frames * a.channels + c0 + sc;
         for (int64_t t = max(t0, length) + sr; t < min(t0 + a.run, a.frames); t += 8)
-            store_pack<T, 2>(py + t * a.channels, zero, sn);
+            store_pack<T, 2>(pe + t * a.channels, Pack<T, 2>::zero(), sn);
     }
     if (a.state_out != nullptr && split == splits - 1 && live) {
 #pragma unroll
         for (int j = 0; j < NP; ++j)
-            if (q * NP + j < a.states) a.state_out[(clip * a.channels + c0 + ch) * a.states + q * NP + j] = h[j];
+            if (state_of(j) < a.states) a.state_out[(clip * a.channels + cl) * a.states + state_of(j)] = h[j];
     }
+}
+
+// Sum over the four lanes of a quad.
+__device__ __forceinline__ float quad_sum(float v) {
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true));
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true));
+    return v;
 }
 
 // One frame: the same formulas, the state read and written once.  Bytes of the state bound it.
@@ -398,24 +521,28 @@ __global__ __launch_bounds__(kThreads) void selective_step_kernel(ScanArgs a, fl
     Pack<T, 4> bs[NI], cs[NI];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-        const int n = (i * 4 + q) * 4, ne = max(0, min(4, a.states - n));
-        hs[i] = load_pack<float, 4>(ps + n, ne);
-        as[i] = load_pack<float, 4>(pa + n, ne);
-        bs[i] = load_pack<T, 4>(pb + n, ne);
-        cs[i] = load_pack<T, 4>(pc + n, ne);
+        const int n = (i * 4 + q) * 4, ne = min(4, a.states - n);
+        if (ne > 0) {
+            hs[i] = load_pack<float, 4>(ps + n, ne);
+            as[i] = load_pack<float, 4>(pa + n, ne);
+            bs[i] = load_pack<T, 4>(pb + n, ne);
+            cs[i] = load_pack<T, 4>(pc + n, ne);
+        }
     }
     if (a.softplus) d = softplus(d);
     const float v = d * x;
     float y = 0.0f;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-        const int n = (i * 4 + q) * 4, ne = max(0, min(4, a.states - n));
+        const int n = (i * 4 + q) * 4, ne = min(4, a.states - n);
+        if (ne <= 0) continue;
+        float h[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            hs[i].v[e] = fmaf(__builtin_amdgcn_exp2f(d * decay_rate(as[i].v[e])), hs[i].v[e], v * static_cast<float>(bs[i].v[e]));
-            y = e < ne ? fmaf(hs[i].v[e], static_cast<float>(cs[i].v[e]), y) : y;
+            h[e] = fmaf(__builtin_amdgcn_exp2f(d * decay_rate(as[i].get(e))), hs[i].get(e), v * bs[i].get(e));
+            y = e < ne ? fmaf(h[e], cs[i].get(e), y) : y;
         }
-        if (ne > 0) store_pack<float, 4>(ps + n, hs[i], ne);
+        store_pack<float, 4>(ps + n, Pack<float, 4>::from(h), ne);
     }
     y = quad_sum(y);
     if (q == 0) {
@@ -435,12 +562,16 @@ int64_t scan_run(int64_t frames, int splits) {
     return sedmi::ceil_div(sedmi::ceil_div(std::max<int64_t>(frames, 1), splits), kTile) * kTile;
 }
 
+// Runs of the time axis.  Splitting costs a second pass over all but the last run (0.6 of the scan itself), a launch and
+// the joining, so time is only split where workgroups are missing, down to one tile per run and up to four workgroups per
+// compute unit.  Measured, whole against split (N = 16, us): 16 workgroups x 250 frames 30 / 18, 10 x 1000 103 / 22,
+// 64 x 250 30 / 19, 32 x 6000 605 / 107; 256 x 250 32 / 39, 384 x 1000 152 / 169; 8 x 64 10 / 12.  More than 64 runs
+// lose to the joining (4 x 6000: 64 runs 41, 94 runs 47).
 int scan_splits(int64_t clips, int64_t frames, int channels, int groups) {
-    const int64_t have = clips * scan_blocks(channels, groups);
-    if (have >= 512) return 1;
-    const int64_t want = sedmi::ceil_div(1024, std::max<int64_t>(1, have));
-    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({want, frames / 128, 64}));
-    return static_cast<int>(sedmi::ceil_div(std::max<int64_t>(frames, 1), scan_run(frames, static_cast<int>(splits))));
+    const int64_t have = std::max<int64_t>(1, clips * scan_blocks(channels, groups));
+    if (have >= 192 || frames < 128) return 1;
+    const int64_t splits = std::min<int64_t>({sedmi::ceil_div(1024, have), frames / kTile, 64});
+    return static_cast<int>(sedmi::ceil_div(frames, scan_run(frames, static_cast<int>(splits))));
 }
 
 bool dtype_ok(int dtype) {

@@ -6,23 +6,71 @@
 template <typename T>
 constexpr int kVec = 16 / static_cast<int>(sizeof(T));
 
-// A row of C elements of an odd C, or of a slice of a projection, starts at any multiple of the element size.  The
-// hardware takes unaligned 16-byte global accesses (gfx950 under ROCm runs with unaligned access on), so one code
-// path serves every alignment: the type below only promises the alignment of an element.
+// Two 16-bit elements of a word, or one float32 word.
+template <typename T>
+__device__ __forceinline__ float element(uint32_t w, int i);
+template <>
+__device__ __forceinline__ float element<float>(uint32_t w, int) { return __builtin_bit_cast(float, w); }
+template <>
+__device__ __forceinline__ float element<__bf16>(uint32_t w, int i) {
+    return __builtin_bit_cast(float, i ? w & 0xffff0000u : w << 16);
+}
+template <>
+__device__ __forceinline__ float element<_Float16>(uint32_t w, int i) {
+    return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(i ? w >> 16 : w)));
+}
+
+// V elements as the 32-bit words they are in memory: unpacked where they are used, so that a row in flight costs no more
+// registers than it has bytes.  A row of an odd number of elements, or of a slice of a projection, starts at any multiple
+// of the element size.  The hardware takes unaligned 16-byte global accesses (gfx950 under ROCm runs with unaligned
+// access on), so one code path serves every alignment: the type only promises the alignment of an element.
 template <typename T, int V>
 struct __attribute__((packed, aligned(sizeof(T)))) Pack {
-    T v[V];
+    static constexpr int kPer = 4 / static_cast<int>(sizeof(T));         // elements per word
+    uint32_t w[V / kPer];
+
+    __device__ __forceinline__ float get(int e) const { return element<T>(w[e / kPer], e % kPer); }
+    __device__ __forceinline__ static Pack zero() {
+        Pack r;
+#pragma unroll
+        for (int i = 0; i < V / kPer; ++i) r.w[i] = 0;
+        return r;
+    }
+    // word i from its elements, rounded to nearest even
+    __device__ __forceinline__ void set_word(int i, const float *v) {
+        if constexpr (kPer == 1) {
+            w[i] = __builtin_bit_cast(uint32_t, v[0]);
+        } else {
+            using F2 = __attribute__((ext_vector_type(2))) float;
+            using T2 = __attribute__((ext_vector_type(2))) T;
+            w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((F2{v[0], v[1]}), T2));
+        }
+    }
+    __device__ __forceinline__ static Pack from(const float *v) {
+        Pack r;
+#pragma unroll
+        for (int i = 0; i < V / kPer; ++i) r.set_word(i, v + i * kPer);
+        return r;
+    }
 };
 
-// The first n of V elements at p (n >= V: all of them in one load); the others are zero and never read.
+template <typename T>
+using Bits = std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t>;
+
+// The first n of V elements at p, 1 <= n: one load, or for the last elements of a row single loads of which those past
+// the end repeat the last element (no branch each, so all are in flight together; what they hold is never stored).
 template <typename T, int V>
 __device__ __forceinline__ Pack<T, V> load_pack(const T *p, int n) {
     Pack<T, V> r;
     if (n >= V) {
         r = *reinterpret_cast<const Pack<T, V> *>(p);
     } else {
+        const Bits<T> *b = reinterpret_cast<const Bits<T> *>(p);
 #pragma unroll
-        for (int e = 0; e < V; ++e) r.v[e] = e < n ? p[e] : static_cast<T>(0.0f);
+        for (int i = 0; i < V / r.kPer; ++i) {
+            r.w[i] = b[min(i * r.kPer, n - 1)];
+            if constexpr (sizeof(T) == 2) r.w[i] |= static_cast<uint32_t>(b[min(2 * i + 1, n - 1)]) << 16;
+        }
     }
     return r;
 }
@@ -32,9 +80,10 @@ __device__ __forceinline__ void store_pack(T *p, const Pack<T, V> &r, int n) {
     if (n >= V) {
         *reinterpret_cast<Pack<T, V> *>(p) = r;
     } else {
+        Bits<T> *b = reinterpret_cast<Bits<T> *>(p);
 #pragma unroll
         for (int e = 0; e < V; ++e)
-            if (e < n) p[e] = r.v[e];
+            if (e < n) b[e] = static_cast<Bits<T>>(r.w[e / r.kPer] >> (sizeof(T) == 2 ? 16 * (e % 2) : 0));
     }
 }
 
