@@ -448,7 +448,7 @@ int sedmi_confusion_counts(const float *p, const float *labels, int64_t n_rows, 
 /* y = act((x - mean) / sqrt(var + eps) * weight[c] + bias[c]) with mean and
  * biased variance over the valid frames, all inner positions and the
  * channels / groups channels of a clip's group.
- *   x, y         device [n_clips, frames, inner, channels], contiguous; y may be x
+ *   x, y         device [n_clips, frames, inner, channels], contiguous; y must not overlap x
  *   weight, bias device float32 [channels] or NULL (1 and 0)
  *   ws           device scratch >= sedmi_group_norm_workspace_bytes() */
 size_t sedmi_group_norm_workspace_bytes(int64_t n_clips, int64_t frames, int64_t inner, int channels, int groups,

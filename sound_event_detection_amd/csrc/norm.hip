@@ -14,6 +14,8 @@ namespace {
 #include "vec_io.h"
 
 constexpr int kThreads = 256;
+constexpr int kMaxChunks = 256;         // of a clip's rows
+constexpr int kUnroll = 4;               // rows of a thread in flight
 
 struct NormArgs {
     const float *weight, *bias;          // [channels] or null
@@ -25,12 +27,37 @@ struct NormArgs {
     // two-launch form
     int groups_per_block, column_blocks, chunks;
     int64_t rows_per_chunk;
+    // one-launch form
+    int vectors;                         // of a row of the group
+    uint32_t per_row_inverse;            // floor(2^32 / vectors) + 1 (vectors > 1): i / vectors for i < 2^16
     float *partial;                      // [clips][chunks][groups][3] = count, mean, sum of squares about the mean
 };
 
-template <typename T>
+// Rows row, row + step, ... of `count` left from row on.
+__device__ __forceinline__ int64_t rows_of(int64_t count, int step) { return count > 0 ? (count + step - 1) / step : 0; }
+
+// Vectors side by side over `width` channels.  The last one of a width that is no multiple of V moves back over its
+// neighbour's channels, `skip` of which it does not count; both write the same values there.  TINY (a width below V): one
+// vector, loaded and stored by element.
+template <typename T, bool TINY>
+struct Column {
+    static constexpr int V = kVec<T>;
+    int at, skip, size;
+    __device__ __forceinline__ Column(int j, int width) : at(TINY ? 0 : min(j * V, width - V)), skip(j * V - at), size(TINY ? width : V) {}
+    __device__ __forceinline__ Pack<T, V> load(const T *p) const { return load_pack<T, V>(p + at, size); }
+    __device__ __forceinline__ void store(T *p, const Pack<T, V> &v) const { store_pack<T, V>(p + at, v, size); }
+    __device__ __forceinline__ bool counts(int e) const { return e >= skip && e < size; }
+};
+
+// --- two launches: statistics of row chunks, then their join and the rows themselves
+//
+// A thread keeps a running mean and a running sum of squares about it per channel (mean += d / n, m2 += d (x - mean)),
+// which loses nothing where the mean is far from zero; one more operation per element than plain sums, in a kernel that
+// waits for memory.  The rows are read twice, the second time mostly from the last-level cache.
+template <typename T, bool TINY>
 __global__ __launch_bounds__(kThreads) void norm_stats_kernel(const T *x, NormArgs a) {
     constexpr int V = kVec<T>;
+    // where vectors lie within a group: one entry per thread; else one per (row lane, channel)
     __shared__ float s_mean[kThreads * V], s_m2[kThreads * V], s_cnt[kThreads];
     const int tid = threadIdx.x;
     const int block = blockIdx.x % a.column_blocks;
@@ -48,67 +75,88 @@ __global__ __launch_bounds__(kThreads) void norm_stats_kernel(const T *x, NormAr
     const int lanes = min(nv, kThreads);                        // threads side by side along a row
     const int rp = kThreads / lanes;
     const int row = tid / lanes, col = tid - row * lanes;
-    float total_n = 0.0f, total_mean = 0.0f, total_m2 = 0.0f;   // one group wider than the workgroup: merged over its columns
-    for (int j = col; j < nv; j += lanes) {
-        const int ne = min(V, width - j * V);
+    const bool inside = ng == 1 || a.per_group % V == 0;        // always so where nv > kThreads (then ng == 1)
+    float total_n = 0.0f, total_mean = 0.0f, total_m2 = 0.0f;
+    for (int j = col; j < nv && row < rp; j += lanes) {
+        const Column<T, TINY> c(j, width);
         float mean[V], m2[V], n = 0.0f;
 #pragma unroll
         for (int e = 0; e < V; ++e) mean[e] = m2[e] = 0.0f;
-        if (row < rp) {
-            for (int64_t r = r0 + row; r < r1; r += rp) {
-                const auto p = load_pack<T, V>(base + r * a.channels + j * V, ne);
-                n += 1.0f;
-                const float inv = __builtin_amdgcn_rcpf(n);
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float v = p.get(e), d = v - mean[e];
-                    mean[e] = fmaf(d, inv, mean[e]);
-                    m2[e] = fmaf(d, v - mean[e], m2[e]);
-                }
-            }
-        }
-        if (nv > kThreads) {
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (e < ne && n > 0.0f) {
-                    const float sum = total_n + n, d = mean[e] - total_mean, w = n / sum;
-                    total_mean = fmaf(d, w, total_mean);
-                    total_m2 += m2[e] + d * d * total_n * w;
-                    total_n = sum;
-                }
-        } else if (row < rp) {
+        const T *p = base + (r0 + row) * a.channels;
+        const int64_t stride = static_cast<int64_t>(rp) * a.channels;
+        auto add = [&](const Pack<T, V> &in) __attribute__((always_inline)) {
+            n += 1.0f;
+            const float inv = __builtin_amdgcn_rcpf(n);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                s_mean[(row * nv + j) * V + e] = mean[e];
-                s_m2[(row * nv + j) * V + e] = m2[e];
+                const float v = in.get(e), d = v - mean[e];
+                mean[e] = fmaf(d, inv, mean[e]);
+                m2[e] = fmaf(d, v - mean[e], m2[e]);
             }
-            s_cnt[row * nv + j] = n;
+        };
+        int left = static_cast<int>(rows_of(r1 - r0 - row, rp));
+        for (; left >= kUnroll; left -= kUnroll, p += kUnroll * stride) {
+            Pack<T, V> in[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) in[u] = c.load(p + u * stride);
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) add(in[u]);
+        }
+        if (left > 0) {                                          // the last rows together, the very last repeated
+            Pack<T, V> in[kUnroll - 1];
+#pragma unroll
+            for (int u = 0; u < kUnroll - 1; ++u) in[u] = c.load(p + min(u, left - 1) * stride);
+#pragma unroll
+            for (int u = 0; u < kUnroll - 1; ++u)
+                if (u < left) add(in[u]);
+        }
+        if (inside) {
+            // the channels of the vector joined, all of count n, and those with what the thread has
+            const float m = static_cast<float>(c.size - c.skip);
+            float sum = 0.0f, q = 0.0f;
+#pragma unroll
+            for (int e = 0; e < V; ++e) sum += c.counts(e) ? mean[e] : 0.0f;
+            const float middle = sum / m;
+#pragma unroll
+            for (int e = 0; e < V; ++e) q += c.counts(e) ? fmaf(n * (mean[e] - middle), mean[e] - middle, m2[e]) : 0.0f;
+            const float all = total_n + n * m, d = middle - total_mean, w = all > 0.0f ? n * m / all : 0.0f;
+            total_mean = fmaf(d, w, total_mean);
+            total_m2 += fmaf(d * d, total_n * w, q);
+            total_n = all;
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (c.counts(e)) {
+                    s_mean[row * nv * V + c.at + e] = mean[e];
+                    s_m2[row * nv * V + c.at + e] = m2[e];
+                }
+            if (j == 0) s_cnt[row] = n;
         }
     }
-    int entries = a.per_group, per_row = nv * V, rows_in = rp;  // entries of one group in a row of the tables
-    if (nv > kThreads) {
-        s_mean[tid] = total_mean, s_m2[tid] = total_m2, s_cnt[tid] = total_n;
-        entries = kThreads, per_row = kThreads, rows_in = 1;
+    // a group's entries: `entries` adjacent ones in each of `rows_in` rows of per_row
+    int entries = a.per_group, per_row = nv * V, rows_in = rp;
+    if (inside) {
+        if (row < rp) s_mean[tid] = total_mean, s_m2[tid] = total_m2, s_cnt[tid] = total_n;
+        entries = ng == 1 ? lanes : a.per_group / V, per_row = lanes;
     }
     __syncthreads();
     const int lane = tid & 63, wave = tid >> 6;
-    for (int g = wave; g < ng; g += kThreads / 64) {
-        float sum = 0.0f, cnt = 0.0f;
-        for (int i = lane; i < entries * rows_in; i += 64) {
-            const int r = i / entries, at = r * per_row + g * entries + (i - r * entries);
-            const float n = nv > kThreads ? s_cnt[at] : s_cnt[at / V];
-            cnt += n;
-            sum = fmaf(n, s_mean[at], sum);
+    const int first_r = lane / entries, first_e = lane - first_r * entries, step_r = 64 / entries, step_e = 64 - step_r * entries;
+    auto walk = [&](int g, auto f) __attribute__((always_inline)) {
+        for (int r = first_r, e = first_e; r < rows_in;) {
+            const int at = r * per_row + g * entries + e;
+            f(at, s_cnt[inside ? at : r]);
+            r += step_r, e += step_e;
+            if (e >= entries) e -= entries, ++r;
         }
+    };
+    for (int g = wave; g < ng; g += kThreads / 64) {
+        float sum = 0.0f, cnt = 0.0f, m2 = 0.0f;
+        walk(g, [&](int at, float n) { cnt += n, sum = fmaf(n, s_mean[at], sum); });
 #pragma unroll
         for (int m = 32; m; m >>= 1) cnt += __shfl_xor(cnt, m), sum += __shfl_xor(sum, m);
         const float mean = cnt > 0.0f ? sum / cnt : 0.0f;
-        float m2 = 0.0f;
-        for (int i = lane; i < entries * rows_in; i += 64) {
-            const int r = i / entries, at = r * per_row + g * entries + (i - r * entries);
-            const float n = nv > kThreads ? s_cnt[at] : s_cnt[at / V], d = s_mean[at] - mean;
-            m2 += s_m2[at] + n * d * d;
-        }
+        walk(g, [&](int at, float n) { m2 += fmaf(n * (s_mean[at] - mean), s_mean[at] - mean, s_m2[at]); });
 #pragma unroll
         for (int m = 32; m; m >>= 1) m2 += __shfl_xor(m2, m);
         if (lane == 0) {
@@ -118,7 +166,7 @@ __global__ __launch_bounds__(kThreads) void norm_stats_kernel(const T *x, NormAr
     }
 }
 
-template <typename T>
+template <typename T, bool TINY, int ACT>
 __global__ __launch_bounds__(kThreads) void norm_apply_kernel(const T *x, T *y, NormArgs a) {
     constexpr int V = kVec<T>;
     __shared__ float s_mean[kThreads * V], s_rstd[kThreads * V];
@@ -135,18 +183,37 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(const T *x, T *y, 
     const int64_t r0 = chunk * a.rows_per_chunk, r1 = min(a.rows, r0 + a.rows_per_chunk);
     const int64_t at0 = clip * a.rows * a.channels + static_cast<int64_t>(g0) * a.per_group;
 
+    const int lanes = min(nv, kThreads);
+    const int rp = kThreads / lanes;
+    const int row = tid / lanes, col = tid - row * lanes;
+    const int64_t stride = static_cast<int64_t>(rp) * a.channels, from = at0 + (r0 + row) * a.channels;
+    const int rows = row < rp ? static_cast<int>(rows_of(r1 - r0 - row, rp)) : 0;
+    const int good = row < rp ? static_cast<int>(rows_of(min(valid, r1) - r0 - row, rp)) : 0;
+    Pack<T, V> in[kUnroll];
+    auto fetch = [&](const Column<T, TINY> &c, int r) __attribute__((always_inline)) {       // rows past the last repeat it
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) in[u] = c.load(x + from + min(r + u, good - 1) * stride);
+    };
+    if (good > 0) fetch(Column<T, TINY>(col, width), 0);         // under way while the statistics are joined
+
     const int lane = tid & 63, wave = tid >> 6;
-    for (int g = wave; g < ng; g += kThreads / 64) {             // chunks <= 64: one lane each
-        float n = 0.0f, m = 0.0f, q = 0.0f;
-        if (lane < a.chunks) {
-            const float *p = a.partial + ((clip * a.chunks + lane) * a.groups + g0 + g) * 3;
-            n = p[0], m = p[1], q = p[2];
+    for (int g = wave; g < ng; g += kThreads / 64) {
+        constexpr int J = kMaxChunks / 64;                       // chunks of a lane
+        float n[J], m[J], q[J], cnt = 0.0f, sum = 0.0f, m2 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < J; ++i) {
+            const bool on = lane + 64 * i < a.chunks;
+            const float *p = a.partial + ((clip * a.chunks + min(lane + 64 * i, a.chunks - 1)) * a.groups + g0 + g) * 3;
+            n[i] = p[0], m[i] = p[1], q[i] = p[2];
+            if (!on) n[i] = m[i] = q[i] = 0.0f;
         }
-        float cnt = n, sum = n * m;
+#pragma unroll
+        for (int i = 0; i < J; ++i) cnt += n[i], sum = fmaf(n[i], m[i], sum);
 #pragma unroll
         for (int k = 32; k; k >>= 1) cnt += __shfl_xor(cnt, k), sum += __shfl_xor(sum, k);
         const float mean = cnt > 0.0f ? sum / cnt : 0.0f;
-        float m2 = q + n * (m - mean) * (m - mean);
+#pragma unroll
+        for (int i = 0; i < J; ++i) m2 += fmaf(n[i] * (m[i] - mean), m[i] - mean, q[i]);
 #pragma unroll
         for (int k = 32; k; k >>= 1) m2 += __shfl_xor(m2, k);
         if (lane == 0) {
@@ -156,32 +223,122 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(const T *x, T *y, 
     }
     __syncthreads();
 
-    const int lanes = min(nv, kThreads);
-    const int rp = kThreads / lanes;
-    const int row = tid / lanes, col = tid - row * lanes;
-    if (row >= rp) return;
-    for (int j = col; j < nv; j += lanes) {
-        const int ne = min(V, width - j * V);
+    for (int j = col; j < nv && rows > 0; j += lanes) {
+        const Column<T, TINY> c(j, width);
+        if (j != col && good > 0) fetch(c, 0);
         float mean[V], scale[V], shift[V];
+        const auto w = a.weight ? load_pack<float, V>(a.weight + g0 * a.per_group + c.at, c.size) : Pack<float, V>::zero();
+        const auto b = a.bias ? load_pack<float, V>(a.bias + g0 * a.per_group + c.at, c.size) : Pack<float, V>::zero();
+        int g = c.at / a.per_group, next = (g + 1) * a.per_group - c.at;     // the element at which the next group begins
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const int c = min(j * V + e, width - 1), g = c / a.per_group, ch = g0 * a.per_group + c;
+            if (e == next && g + 1 < ng) ++g, next += a.per_group;
             mean[e] = s_mean[g];
-            scale[e] = s_rstd[g] * (a.weight ? a.weight[ch] : 1.0f);
-            shift[e] = a.bias ? a.bias[ch] : 0.0f;
+            scale[e] = s_rstd[g] * (a.weight ? w.get(e) : 1.0f);
+            shift[e] = b.get(e);
         }
-        for (int64_t r = r0 + row; r < r1; r += rp) {
-            const int64_t at = at0 + r * a.channels + j * V;
-            Pack<T, V> out = Pack<T, V>::zero();
-            if (r < valid) {
-                const auto p = load_pack<T, V>(x + at, ne);
+        for (int r = 0; r < good; r += kUnroll) {
+            Pack<T, V> out[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
                 float v[V];
 #pragma unroll
-                for (int e = 0; e < V; ++e) v[e] = activate(fmaf(p.get(e) - mean[e], scale[e], shift[e]), a.act);
-                out = Pack<T, V>::from(v);
+                for (int e = 0; e < V; ++e)
+                    v[e] = activate(fmaf(in[u].get(e) - mean[e], scale[e], shift[e]), ACT < 0 ? a.act : ACT);
+                out[u] = Pack<T, V>::from(v);
             }
-            store_pack<T, V>(y + at, out, ne);
+            if (r + kUnroll < good) fetch(c, r + kUnroll);
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u)
+                if (r + u < good) c.store(y + from + (r + u) * stride, out[u]);
         }
+        for (int r = good; r < rows; ++r) c.store(y + from + r * stride, Pack<T, V>::zero());
+    }
+}
+
+// --- one launch: a clip's group of at least V channels fits into the registers of a workgroup
+//
+// x is read once and held as it is in memory; mean, then the squares about it, then the output.  Workgroups of the groups
+// of one clip follow each other on one die (blocks are dealt to the 8 dies in turn), so lines that two groups share are
+// fetched into one L2.
+template <typename T, int N, int ACT>
+__global__ __launch_bounds__(1024) void norm_slab_kernel(const T *x, T *y, NormArgs a) {
+    constexpr int V = kVec<T>;
+    __shared__ float s_sum[2][16];
+    const int tid = threadIdx.x, threads = blockDim.x;
+    const unsigned per_die = gridDim.x / 8, dealt = per_die * 8;
+    const unsigned block = blockIdx.x < dealt ? (blockIdx.x % 8) * per_die + blockIdx.x / 8 : blockIdx.x;
+    const int64_t clip = block / a.groups;
+    const int c0 = (block - static_cast<unsigned>(clip) * a.groups) * a.per_group;
+    const int rows = static_cast<int>(a.rows);
+    const int good = static_cast<int>(clamp_length(a.lengths, clip, a.frames) * a.inner);       // valid rows
+    const T *px = x + clip * a.rows * a.channels + c0;
+    T *py = y + clip * a.rows * a.channels + c0;
+
+    auto row_of = [&](int k) __attribute__((always_inline)) {
+        const unsigned i = tid + k * threads;
+        return static_cast<int>(a.vectors == 1 ? i : __umulhi(i, a.per_row_inverse));
+    };
+    auto column_of = [&](int k, int row) __attribute__((always_inline)) {
+        return Column<T, false>(tid + k * threads - row * a.vectors, a.per_group);
+    };
+    Pack<T, V> in[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int row = row_of(k);
+        in[k] = Pack<T, V>::zero();
+        if (row < good) in[k] = column_of(k, row).load(px + static_cast<int64_t>(row) * a.channels);
+    }
+    // unpacked anew in each phase: kept as float32 between them, the rows would need twice the registers
+    auto repack = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int i = 0; i < V / Pack<T, V>::kPer; ++i) asm volatile("" : "+v"(in[k].w[i]));
+    };
+    auto total = [&](float v, float *s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
+        if ((tid & 63) == 0) s[tid >> 6] = v;
+        __syncthreads();
+        float t = 0.0f;
+        for (int i = 0; i < threads / 64; ++i) t += s[i];
+        return t;
+    };
+    float sum = 0.0f, squares = 0.0f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int skip = column_of(k, row_of(k)).skip;
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum += e >= skip ? in[k].get(e) : 0.0f;
+    }
+    const float items = fmaxf(static_cast<float>(good) * static_cast<float>(a.per_group), 1.0f);
+    const float mean = total(sum, s_sum[0]) / items;
+    repack();
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int row = row_of(k), skip = row < good ? column_of(k, row).skip : V;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float d = in[k].get(e) - mean;
+            squares += e >= skip ? d * d : 0.0f;
+        }
+    }
+    const float rstd = 1.0f / sqrtf(total(squares, s_sum[1]) / items + a.eps);
+    repack();
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int row = row_of(k);
+        if (row >= rows) continue;
+        const auto c = column_of(k, row);
+        Pack<float, V> w, b = Pack<float, V>::zero();
+        if (a.weight) w = load_pack<float, V>(a.weight + c0 + c.at, V);
+        if (a.bias) b = load_pack<float, V>(a.bias + c0 + c.at, V);
+        float v[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            v[e] = activate(fmaf((in[k].get(e) - mean) * rstd, a.weight ? w.get(e) : 1.0f, b.get(e)), ACT < 0 ? a.act : ACT);
+        c.store(py + static_cast<int64_t>(row) * a.channels, row < good ? Pack<T, V>::from(v) : Pack<T, V>::zero());
     }
 }
 
@@ -189,6 +346,7 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(const T *x, T *y, 
 struct NormPlan {
     int groups_per_block, column_blocks, chunks;
     int64_t rows_per_chunk;
+    bool tiny;                           // the narrowest block has fewer channels than a vector
 };
 
 NormPlan norm_plan(int64_t clips, int64_t rows, int channels, int groups, int vec) {
@@ -196,22 +354,52 @@ NormPlan norm_plan(int64_t clips, int64_t rows, int channels, int groups, int ve
     const int per_group = channels / groups;
     p.groups_per_block = std::max(1, std::min(groups, kThreads * vec / per_group));
     p.column_blocks = static_cast<int>(sedmi::ceil_div(groups, p.groups_per_block));
+    p.groups_per_block = static_cast<int>(sedmi::ceil_div(groups, p.column_blocks));         // blocks of nearly one width
+    p.column_blocks = static_cast<int>(sedmi::ceil_div(groups, p.groups_per_block));
+    p.tiny = (groups - (p.column_blocks - 1) * p.groups_per_block) * per_group < vec;
     const int nv = std::min<int64_t>(kThreads, sedmi::ceil_div(static_cast<int64_t>(p.groups_per_block) * per_group, vec));
     const int64_t rp = kThreads / nv;
-    const int64_t want = sedmi::ceil_div(2048, std::max<int64_t>(1, clips * p.column_blocks));
-    const int64_t most = std::max<int64_t>(1, rows / (rp * 8));
-    p.chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, most, 64})));
+    // Every workgroup joins statistics, so few: two per compute unit (128 x 250 x 8 x 128 with 32 groups, bf16: 512 53 us,
+    // 1024 57, 2048 74), and no less than kUnroll rows for each of its threads.
+    const int64_t want = sedmi::ceil_div(512, std::max<int64_t>(1, clips * p.column_blocks));
+    const int64_t most = std::max<int64_t>(1, rows / (rp * kUnroll));
+    p.chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxChunks})));
     p.rows_per_chunk = sedmi::ceil_div(std::max<int64_t>(rows, 1), p.chunks);
     return p;
 }
 
 int dtype_vec(int dtype) { return dtype == SEDMI_DTYPE_F32 ? 4 : 8; }
 
+// Whether a clip's group is normalised by one workgroup in one launch: up to 64 KiB of it, and up to 128 KiB where there
+// are workgroups for every compute unit (a single unit takes 5 us for the second 64 KiB).  Measured, one launch against two
+// (us): 64 x 32 groups of 16 kB bf16 19.2 / 59, 1 x 64 KiB 8.9 / 9.2, 128 x 64 KiB 10.4 / 12.2, 64 x 128 KiB 16.0 / 12.3,
+// 256 x 128 KiB 21.2 / 22.4, 1024 x 128 KiB f32 81 / 86, 64 x 256 KiB 28 / 16.
+bool use_slab(int64_t clips, int64_t rows, int channels, int groups, int vec) {
+    const int per_group = channels / groups;
+    const int64_t vectors = rows * sedmi::ceil_div(per_group, vec);
+    return per_group >= vec && (vectors <= 4096 || (vectors <= 8192 && clips * groups >= 256));
+}
+
+template <typename T>
+void launch_slab(const T *x, T *y, NormArgs a, int64_t clips, hipStream_t st) {
+    a.vectors = static_cast<int>(sedmi::ceil_div(a.per_group, kVec<T>));
+    a.per_row_inverse = a.vectors > 1 ? static_cast<uint32_t>((uint64_t{1} << 32) / a.vectors + 1) : 0;
+    const int64_t vectors = a.rows * a.vectors;
+    const int threads = vectors <= 512 ? 256 : vectors <= 1024 ? 512 : 1024;       // up to 2 vectors each, then up to 8
+    const unsigned blocks = static_cast<unsigned>(clips * a.groups);
+    with_activation(a.act, [&](auto act) {
+        constexpr int kAct = decltype(act)::value;
+        const int64_t each = sedmi::ceil_div(vectors, threads);
+        if (each <= 1) norm_slab_kernel<T, 1, kAct><<<blocks, threads, 0, st>>>(x, y, a);
+        else if (each <= 2) norm_slab_kernel<T, 2, kAct><<<blocks, threads, 0, st>>>(x, y, a);
+        else if (each <= 4) norm_slab_kernel<T, 4, kAct><<<blocks, threads, 0, st>>>(x, y, a);
+        else norm_slab_kernel<T, 8, kAct><<<blocks, threads, 0, st>>>(x, y, a);
+    });
+}
+
 bool norm_shape_ok(int64_t clips, int64_t frames, int64_t inner, int channels, int groups, int dtype) {
-    return clips >= 0 && frames >= 0 && inner > 0 && channels > 0 && groups > 0 && channels % groups == 0 &&
-           (dtype == SEDMI_DTYPE_F32 || dtype == SEDMI_DTYPE_F16 || dtype == SEDMI_DTYPE_BF16) &&
-           frames <= (int64_t{1} << 40) / inner && frames * inner <= (int64_t{1} << 40) / channels &&
-           clips <= (int64_t{1} << 24);
+    return frames >= 0 && inner > 0 && frames <= (int64_t{1} << 40) / inner &&
+           sequence_shape_ok(clips, frames * inner, channels) && groups > 0 && channels % groups == 0 && dtype_ok(dtype);
 }
 
 }  // namespace
@@ -221,6 +409,7 @@ extern "C" {
 size_t sedmi_group_norm_workspace_bytes(int64_t n_clips, int64_t frames, int64_t inner, int channels, int groups,
                                         int dtype) {
     if (!norm_shape_ok(n_clips, frames, inner, channels, groups, dtype)) return 0;
+    if (use_slab(n_clips, frames * inner, channels, groups, dtype_vec(dtype))) return 0;
     const NormPlan p = norm_plan(n_clips, frames * inner, channels, groups, dtype_vec(dtype));
     return static_cast<size_t>(n_clips) * p.chunks * groups * 3 * sizeof(float);
 }
@@ -242,6 +431,19 @@ int sedmi_group_norm(const void *x, const float *weight, const float *bias, cons
     a.frames = frames, a.inner = inner, a.rows = frames * inner;
     a.channels = channels, a.groups = groups, a.per_group = channels / groups;
     a.eps = eps, a.act = activation;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const double items = static_cast<double>(n_clips) * a.rows * channels;
+    const double es = dtype == SEDMI_DTYPE_F32 ? 4 : 2;
+    if (use_slab(n_clips, a.rows, channels, groups, dtype_vec(dtype))) {
+        SEDMI_REQUIRE(n_clips * groups < (int64_t{1} << 31), "group_norm: too many workgroups");
+        sedmi::ProfileScope scope("norm_slab_kernel", st, 8 * items, 2 * es * items);
+        with_dtype(dtype, [&](auto t) -> int {
+            launch_slab(static_cast<const decltype(t) *>(x), static_cast<decltype(t) *>(y), a, n_clips, st);
+            return SEDMI_OK;
+        });
+        SEDMI_CHECK_LAUNCH();
+        return SEDMI_OK;
+    }
     const NormPlan p = norm_plan(n_clips, a.rows, channels, groups, dtype_vec(dtype));
     a.groups_per_block = p.groups_per_block, a.column_blocks = p.column_blocks;
     a.chunks = p.chunks, a.rows_per_chunk = p.rows_per_chunk;
@@ -251,20 +453,26 @@ int sedmi_group_norm(const void *x, const float *weight, const float *bias, cons
     if (ws == nullptr || ws_bytes < need)
         return sedmi::set_error(SEDMI_ENOMEM, "group_norm: workspace of %zu bytes, %zu needed", ws_bytes, need);
     a.partial = static_cast<float *>(ws);
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    const double items = static_cast<double>(n_clips) * a.rows * channels;
-    const double es = dtype == SEDMI_DTYPE_F32 ? 4 : 2;
+    const unsigned grid = static_cast<unsigned>(blocks);
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
+        const T *px = static_cast<const T *>(x);
+        T *py = static_cast<T *>(y);
         {
             sedmi::ProfileScope scope("norm_stats_kernel", st, 4 * items, es * items);
-            norm_stats_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(static_cast<const T *>(x), a);
+            if (p.tiny) norm_stats_kernel<T, true><<<grid, kThreads, 0, st>>>(px, a);
+            else norm_stats_kernel<T, false><<<grid, kThreads, 0, st>>>(px, a);
         }
         SEDMI_CHECK_LAUNCH();
         {
             sedmi::ProfileScope scope("norm_apply_kernel", st, 4 * items, 2 * es * items);
-            norm_apply_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(static_cast<const T *>(x),
-                                                                                      static_cast<T *>(y), a);
+            if (p.tiny) {
+                norm_apply_kernel<T, true, -1><<<grid, kThreads, 0, st>>>(px, py, a);
+            } else {
+                with_activation(activation, [&](auto act) {
+                    norm_apply_kernel<T, false, decltype(act)::value><<<grid, kThreads, 0, st>>>(px, py, a);
+                });
+            }
         }
         SEDMI_CHECK_LAUNCH();
         return SEDMI_OK;

@@ -1,5 +1,5 @@
-// Linear sequence mixers of a frame classifier on channels-last frames [clips, frames, channels]: the short causal
-// convolution and the selective state space scan behind it, over whole recordings and one frame at a time.
+// Selective state space scan over channels-last frames [clips, frames, channels], over whole recordings and one frame at
+// a time: the linear recurrence of a frame classifier.
 #include "common.h"
 
 #include <algorithm>
@@ -9,145 +9,6 @@ namespace {
 #include "vec_io.h"
 
 constexpr int kThreads = 256;
-
-// ------------------------------------------------------------------------------------------------ causal convolution
-// y[t, c] = act(bias[c] + sum_k weight[c, k] x[t - (K-1) + k, c]), x before the first frame from the state.
-//
-// Bytes bound it: x is read once and y written once.  A lane owns 16 bytes of channels and walks kRows frames with
-// the last K-1 inputs in registers, so only the K-1 rows in front of each run are read twice.
-struct ConvArgs {
-    const float *weight, *bias;          // [channels, K], [channels] or null
-    const int64_t *lengths;              // [clips] or null
-    int64_t x_clip, x_frame;             // strides of x in elements
-    int64_t frames, clips;
-    int channels, vectors;               // vectors = 16-byte vectors of a row
-    int segments, rows;                  // runs of `rows` frames per clip
-    int act, reverse;
-    uint32_t blocks_per_clip;
-};
-
-template <typename T, int K>
-__global__ __launch_bounds__(kThreads) void causal_conv_kernel(const T *x, const T *state_in, T *state_out, T *y,
-                                                               ConvArgs a) {
-    constexpr int V = kVec<T>, H = K - 1, U = 4;
-    const int64_t clip = blockIdx.x / a.blocks_per_clip;
-    const int64_t item = static_cast<int64_t>(blockIdx.x % a.blocks_per_clip) * kThreads + threadIdx.x;
-    const int segment = static_cast<int>(item / a.vectors);
-    if (segment >= a.segments) return;
-    const int c0 = static_cast<int>(item - static_cast<int64_t>(segment) * a.vectors) * V;
-    const int ne = min(V, a.channels - c0);
-    const int64_t length = clamp_length(a.lengths, clip, a.frames);
-    // frame t of the processing order is row t, or row length-1-t of a reversed clip
-    const T *px = x + clip * a.x_clip + (a.reverse && length > 0 ? (length - 1) * a.x_frame : 0) + c0;
-    T *py = y + (clip * a.frames + (a.reverse && length > 0 ? length - 1 : 0)) * a.channels + c0;
-    const int64_t sx = a.reverse ? -a.x_frame : a.x_frame, sy = a.reverse ? -a.channels : a.channels;
-    const int64_t state_at = clip * H * a.channels + c0;
-
-    // the V x K weights of these channels are adjacent
-    Pack<float, 4> wp[V * K / 4], bp[V / 4];
-#pragma unroll
-    for (int i = 0; i < V * K / 4; ++i)
-        wp[i] = load_pack<float, 4>(a.weight + static_cast<int64_t>(c0) * K + min(4 * i, ne * K - 1), ne * K - 4 * i);
-#pragma unroll
-    for (int i = 0; i < V / 4; ++i)
-        bp[i] = a.bias ? load_pack<float, 4>(a.bias + c0 + min(4 * i, ne - 1), ne - 4 * i) : Pack<float, 4>::zero();
-    auto w = [&](int e, int k) { return wp[(e * K + k) / 4].get((e * K + k) % 4); };
-    const int64_t t0 = static_cast<int64_t>(segment) * a.rows, t1 = min(t0 + a.rows, a.frames), tv = min(t1, length);
-    Pack<T, V> win[H + U];                                       // the inputs as they are: H past ones, then U new ones
-#pragma unroll
-    for (int i = 0; i < H; ++i) {
-        const int64_t t = t0 - H + i;                            // rows >= H: a later run never reaches the state
-        if (t >= 0 && t < length) {
-            win[i] = load_pack<T, V>(px + t * sx, ne);
-        } else if (t < 0 && state_in != nullptr) {
-            win[i] = load_pack<T, V>(state_in + state_at + static_cast<int64_t>(i) * a.channels, ne);
-        } else {
-            win[i] = Pack<T, V>::zero();
-        }
-    }
-    if (segment == 0 && state_out != nullptr) {
-        // the last H inputs of (state, valid frames), oldest first; this lane alone looks at its channels of the state
-        // and has read them, so state_out may be state_in
-        Pack<T, V> last[H > 0 ? H : 1];
-#pragma unroll
-        for (int i = 0; i < H; ++i) {
-            const int64_t t = length - H + i;
-            if (t >= 0) {
-                last[i] = load_pack<T, V>(px + t * sx, ne);
-            } else {
-                last[i] = win[0];
-#pragma unroll
-                for (int k = 1; k < H; ++k)
-                    if (t + H == k) last[i] = win[k];
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < H; ++i)
-            store_pack<T, V>(state_out + state_at + static_cast<int64_t>(i) * a.channels, last[i], ne);
-    }
-    auto fetch = [&](int64_t t, Pack<T, V> *to) {                // frames behind the end repeat the last one
-#pragma unroll
-        for (int u = 0; u < U; ++u) to[u] = load_pack<T, V>(px + min(t + u, tv - 1) * sx, ne);
-    };
-    Pack<T, V> next[U];
-    if (t0 < tv) fetch(t0, next);
-    for (int64_t t = t0; t < tv; t += U) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) win[H + u] = next[u];
-        if (t + U < tv) fetch(t + U, next);
-        Pack<T, V> out[U];
-        constexpr int P = Pack<T, V>::kPer;
-#pragma unroll
-        for (int i = 0; i < V / P; ++i) {                        // a word of channels at a time
-            float s[U][P];
-#pragma unroll
-            for (int e = 0; e < P; ++e) {
-                float f[H + U];
-#pragma unroll
-                for (int r = 0; r < H + U; ++r) f[r] = win[r].get(i * P + e);
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    float v = bp[(i * P + e) / 4].get((i * P + e) % 4);
-#pragma unroll
-                    for (int k = 0; k < K; ++k) v = fmaf(w(i * P + e, k), f[u + k], v);
-                    s[u][e] = activate(v, a.act);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) out[u].set_word(i, s[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (t + u < tv) store_pack<T, V>(py + (t + u) * sy, out[u], ne);
-#pragma unroll
-        for (int i = 0; i < H; ++i) win[i] = win[U + i];
-    }
-    for (int64_t t = max(t0, length); t < t1; ++t)
-        store_pack<T, V>(y + (clip * a.frames + t) * a.channels + c0, Pack<T, V>::zero(), ne);
-}
-
-constexpr int kMaxWidth = 8;
-
-template <typename T>
-int launch_conv(int width, unsigned blocks, hipStream_t st, const void *x, const void *si, void *so, void *y,
-                const ConvArgs &a) {
-    auto go = [&](auto k) {
-        causal_conv_kernel<T, decltype(k)::value><<<blocks, kThreads, 0, st>>>(
-            static_cast<const T *>(x), static_cast<const T *>(si), static_cast<T *>(so), static_cast<T *>(y), a);
-    };
-    switch (width) {
-        case 1: go(std::integral_constant<int, 1>{}); break;
-        case 2: go(std::integral_constant<int, 2>{}); break;
-        case 3: go(std::integral_constant<int, 3>{}); break;
-        case 4: go(std::integral_constant<int, 4>{}); break;
-        case 5: go(std::integral_constant<int, 5>{}); break;
-        case 6: go(std::integral_constant<int, 6>{}); break;
-        case 7: go(std::integral_constant<int, 7>{}); break;
-        default: go(std::integral_constant<int, 8>{}); break;
-    }
-    SEDMI_CHECK_LAUNCH();
-    return SEDMI_OK;
-}
 
 // ----------------------------------------------------------------------------------------------------- selective scan
 //     d_t = softplus(dt_t + dt_bias)        (or dt_t + dt_bias)
@@ -574,13 +435,9 @@ int scan_splits(int64_t clips, int64_t frames, int channels, int groups) {
     return static_cast<int>(sedmi::ceil_div(frames, scan_run(frames, static_cast<int>(splits))));
 }
 
-bool dtype_ok(int dtype) {
-    return dtype == SEDMI_DTYPE_F32 || dtype == SEDMI_DTYPE_F16 || dtype == SEDMI_DTYPE_BF16;
-}
-
 bool scan_shape_ok(int64_t clips, int64_t frames, int channels, int groups, int states) {
-    return clips >= 0 && clips <= (int64_t{1} << 24) && frames >= 0 && frames <= (int64_t{1} << 40) && channels > 0 &&
-           channels <= (1 << 24) && groups > 0 && channels % groups == 0 && states > 0 && states <= kMaxStates;
+    return sequence_shape_ok(clips, frames, channels) && groups > 0 && channels % groups == 0 && states > 0 &&
+           states <= kMaxStates;
 }
 
 int check_scan(const sedmi_scan_args *p, const char *who) {
@@ -628,49 +485,9 @@ void launch_step(int states, unsigned blocks, hipStream_t st, const ScanArgs &a,
     else selective_step_kernel<T, 8><<<blocks, kThreads, 0, st>>>(a, state);
 }
 
-bool overlap(const void *p, const void *q, size_t bytes) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(q);
-    return p != nullptr && q != nullptr && x < y + bytes && y < x + bytes;
-}
-
 }  // namespace
 
 extern "C" {
-
-int sedmi_causal_conv1d(const void *x, int64_t x_stride_clip, int64_t x_stride_frame, const float *weight,
-                        const float *bias, const int64_t *lengths, const void *state_in, void *state_out, void *y,
-                        int64_t n_clips, int64_t frames, int channels, int width, int activation, int reverse,
-                        int dtype, void *stream) {
-    SEDMI_REQUIRE(dtype_ok(dtype), "causal_conv1d: unknown dtype %d", dtype);
-    SEDMI_REQUIRE(width >= 1 && width <= kMaxWidth, "causal_conv1d: width (%d) must be 1 .. %d", width, kMaxWidth);
-    SEDMI_REQUIRE(activation >= SEDMI_ACT_NONE && activation <= SEDMI_ACT_GELU, "causal_conv1d: unknown activation %d", activation);
-    SEDMI_REQUIRE(scan_shape_ok(n_clips, frames, channels, 1, 1), "causal_conv1d: bad shape (clips %lld, frames %lld, channels %d)",
-                  static_cast<long long>(n_clips), static_cast<long long>(frames), channels);
-    const size_t es = dtype == SEDMI_DTYPE_F32 ? 4 : 2;
-    const size_t state_bytes = static_cast<size_t>(n_clips) * (width - 1) * channels * es;
-    SEDMI_REQUIRE(state_in == state_out || !overlap(state_in, state_out, state_bytes),
-                  "causal_conv1d: state_in and state_out overlap without being the same buffer");
-    if (n_clips == 0) return SEDMI_OK;
-    SEDMI_REQUIRE(weight != nullptr && (frames == 0 || (x != nullptr && y != nullptr)), "causal_conv1d: null x, weight or y");
-    ConvArgs a{};
-    a.weight = weight, a.bias = bias, a.lengths = lengths;
-    a.x_clip = x_stride_clip, a.x_frame = x_stride_frame;
-    a.frames = frames, a.clips = n_clips, a.channels = channels;
-    a.act = activation, a.reverse = reverse != 0;
-    a.vectors = static_cast<int>(sedmi::ceil_div(channels, static_cast<int64_t>(16 / es)));
-    a.rows = 32;
-    const int64_t segments = std::max<int64_t>(1, sedmi::ceil_div(frames, a.rows));      // no frames: the state alone
-    const int64_t per_clip = sedmi::ceil_div(segments * a.vectors, kThreads), blocks = per_clip * n_clips;
-    SEDMI_REQUIRE(segments < (int64_t{1} << 31) && blocks < (int64_t{1} << 31), "causal_conv1d: too many workgroups (%lld)",
-                  static_cast<long long>(blocks));
-    a.segments = static_cast<int>(segments), a.blocks_per_clip = static_cast<uint32_t>(per_clip);
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    const double items = static_cast<double>(n_clips) * frames * channels;
-    sedmi::ProfileScope scope("causal_conv_kernel", st, 2.0 * width * items, 2.0 * es * items);
-    return with_dtype(dtype, [&](auto t) -> int {
-        return launch_conv<decltype(t)>(width, static_cast<unsigned>(blocks), st, x, state_in, state_out, y, a);
-    });
-}
 
 size_t sedmi_selective_scan_workspace_bytes(int64_t n_clips, int64_t frames, int channels, int groups, int states) {
     if (!scan_shape_ok(n_clips, frames, channels, groups, states)) return 0;

@@ -1,4 +1,4 @@
-// Element types and 16-byte row access of the channels-last sequence operators (norm.hip, sequence.hip).  Meant to
+// Element types and 16-byte row access of the channels-last sequence operators (norm.hip, conv1d.hip, scan.hip).  Meant to
 // be included INSIDE an anonymous namespace of the including translation unit.
 #pragma once
 
@@ -103,10 +103,33 @@ __device__ __forceinline__ int64_t clamp_length(const int64_t *lengths, int64_t 
     return n < 0 ? 0 : (n > most ? most : n);
 }
 
+inline bool dtype_ok(int dtype) {
+    return dtype == SEDMI_DTYPE_F32 || dtype == SEDMI_DTYPE_F16 || dtype == SEDMI_DTYPE_BF16;
+}
+
+// Limits that keep every product of the extents below 2^63.
+inline bool sequence_shape_ok(int64_t clips, int64_t frames, int64_t channels) {
+    return clips >= 0 && clips <= (int64_t{1} << 24) && frames >= 0 && frames <= (int64_t{1} << 40) / (channels > 0 ? channels : 1) &&
+           channels > 0 && channels <= (1 << 24);
+}
+
+inline bool overlap(const void *p, const void *q, size_t bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(q);
+    return p != nullptr && q != nullptr && x < y + bytes && y < x + bytes;
+}
+
 // Dispatches f(T{}) on a SEDMI_DTYPE_* code.
 template <typename F>
 int with_dtype(int dtype, F f) {
     if (dtype == SEDMI_DTYPE_F32) return f(float{});
     if (dtype == SEDMI_DTYPE_F16) return f(static_cast<_Float16>(0.0f));
     return f(static_cast<__bf16>(0.0f));
+}
+
+// Calls f with the activation as a constant where it is common (none, silu), with -1 (look it up) otherwise.
+template <typename F>
+void with_activation(int act, F f) {
+    if (act == SEDMI_ACT_NONE) f(std::integral_constant<int, SEDMI_ACT_NONE>{});
+    else if (act == SEDMI_ACT_SILU) f(std::integral_constant<int, SEDMI_ACT_SILU>{});
+    else f(std::integral_constant<int, -1>{});
 }

@@ -9,7 +9,7 @@
 
 They stand beside the models' own stages (BatchNorm inside the conv blocks, GRU recurrences, attention) for frame
 classifiers that normalise without batch statistics and that have to answer frame by frame; the reference has none of
-them.  The arithmetic runs in the HIP kernels of csrc/norm.hip and csrc/sequence.hip through the C ABI
+them.  The arithmetic runs in the HIP kernels of csrc/norm.hip, csrc/conv1d.hip and csrc/scan.hip through the C ABI
 (``sedmi_group_norm``, ``sedmi_causal_conv1d``, ``sedmi_selective_scan``, ``sedmi_selective_step``).  Inference only:
 there is no backward and no CPU path.
 

@@ -31,6 +31,10 @@ NORM_SHAPES = [
     # clips, frames, inner, channels, groups
     (1, 1, 1, 1, 1), (2, 3, 1, 6, 3), (3, 7, 5, 24, 2), (2, 33, 1, 64, 64), (1, 251, 1, 387, 1), (2, 129, 2, 96, 32),
     (5, 40, 3, 40, 5), (2, 9, 1, 2500, 1), (1, 12, 1, 4100, 2), (2, 700, 4, 16, 4), (1, 2100, 1, 256, 8), (3, 50, 1, 7, 7),
+    # groups of more than a workgroup's registers: rows in chunks, one group wider than a workgroup, several column
+    # blocks, groups that end inside a 16-byte vector, rows of fewer channels than a vector
+    (2, 300, 1, 1024, 2), (1, 40, 1, 2500, 1), (1, 60, 1, 4100, 1), (1, 70, 1, 5000, 200), (2, 1100, 1, 60, 10),
+    (3, 500, 1, 37, 37), (2, 9000, 1, 5, 1), (1, 700, 1, 3, 3), (1, 9, 1, 2056, 257), (2, 901, 2, 100, 1),
 ]
 
 

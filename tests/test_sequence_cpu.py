@@ -16,8 +16,8 @@ def lib():
 P = C.c_void_p(4096)            # a pointer that a refused call never follows
 
 
-def norm(lib, x=P, clips=2, frames=3, inner=1, channels=8, groups=2, eps=1e-5, act=0, dtype=0, ws=P, ws_bytes=1 << 20):
-    return lib.sedmi_group_norm(x, None, None, None, x, clips, frames, inner, channels, groups, eps, act, dtype, ws, ws_bytes,
+def norm(lib, x=P, y=C.c_void_p(1 << 40), clips=2, frames=3, inner=1, channels=8, groups=2, eps=1e-5, act=0, dtype=0, ws=P, ws_bytes=1 << 20):
+    return lib.sedmi_group_norm(x, None, None, None, y, clips, frames, inner, channels, groups, eps, act, dtype, ws, ws_bytes,
                                 None)
 
 
