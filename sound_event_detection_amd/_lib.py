@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SEDMI_LIB_PATH") or os.path.join(_HERE, "libsedmi.so")
@@ -87,12 +88,16 @@ ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3
 
 
 class ScanArgs(C.Structure):
+    """sedmi_scan_args.  ``pack_scan_args`` makes the same bytes from its members in order, a microsecond faster."""
     _fields_ = ([(n, C.c_void_p) for n in ("x", "dt", "z", "B", "C", "A", "D", "dt_bias", "lengths", "state_in",
                                            "state_out", "y")]
                 + [(n, C.c_int64 * 2) for n in ("x_stride", "dt_stride", "z_stride")]
                 + [(n, C.c_int64 * 3) for n in ("B_stride", "C_stride")]
                 + [(n, C.c_int64) for n in ("n_clips", "frames")]
                 + [(n, C.c_int) for n in ("channels", "groups", "states", "dtype", "dt_softplus", "reverse")])
+
+
+pack_scan_args = struct.Struct("12Q14q6i").pack     # 12 pointers, 12 strides and 2 extents, 6 ints
 
 
 class KernelStat(C.Structure):
@@ -149,8 +154,8 @@ SIGNATURES = {
     "sedmi_group_norm": (_I, [_VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _I, _I, _F, _I, _I, _VP, _SZ, _VP]),
     "sedmi_causal_conv1d": (_I, [_VP, _I64, _I64, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I, _I, _I, _I, _I, _VP]),
     "sedmi_selective_scan_workspace_bytes": (_SZ, [_I64, _I64, _I, _I, _I]),
-    "sedmi_selective_scan": (_I, [C.POINTER(ScanArgs), _VP, _SZ, _VP]),
-    "sedmi_selective_step": (_I, [C.POINTER(ScanArgs), _VP]),
+    "sedmi_selective_scan": (_I, [_VP, _VP, _SZ, _VP]),      # a ScanArgs by reference, or its bytes
+    "sedmi_selective_step": (_I, [_VP, _VP]),
     "sedmi_profile_enable": (_I, [_I]),
     "sedmi_profile_collect": (_I, [C.POINTER(KernelStat), _I]),
 }
@@ -193,7 +198,8 @@ def ptr(t) -> C.c_void_p:
 def stream_ptr(device) -> C.c_void_p:
     """The hipStream_t torch is currently enqueueing on for ``device``."""
     import torch
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(index))     # 0.1 us; a torch.cuda.Stream object costs 2
 
 
 def profile_enable(on: bool) -> None:

@@ -58,7 +58,7 @@ def _activation(name, who):
 
 def _like(t, x, shape, what):
     """``t`` checked to be of x's type and device and of the given shape, its last dimension adjacent."""
-    if t.dtype != x.dtype or t.device != x.device:
+    if t.dtype is not x.dtype or t.get_device() != x.get_device():
         raise TypeError(f"{what}: {x.dtype} on {x.device} like x, not {t.dtype} on {t.device}")
     if t.shape != shape:
         raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
@@ -66,15 +66,14 @@ def _like(t, x, shape, what):
 
 
 def _param(t, x, shape, what):
+    """``t`` checked to be on x's device and of the given shape, as contiguous float32; None stays."""
     if t is None:
         return None
     if t.shape != shape:
         raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.device != x.device:
+    if t.get_device() != x.get_device():
         raise TypeError(f"{what}: on {t.device}, x is on {x.device}")
-    if t.dtype != torch.float32:
-        t = t.to(torch.float32)
-    return t.contiguous()
+    return t.to(torch.float32).contiguous() if t.dtype is not torch.float32 else t.contiguous()
 
 
 def _lengths(lengths, n, device, who):
@@ -88,18 +87,21 @@ def _lengths(lengths, n, device, who):
     return t.to(device, torch.int64).contiguous()
 
 
-def _call(x, entry, *args):
-    """One entry point on the current stream of x's device, with that device current."""
+def _call(device, entry, *args):
+    """One entry point on the current stream of ``device``, with that device current.  ``args``: numbers, and addresses as
+    ``_address`` gives them."""
     fn = getattr(_lib.lib(), entry)
-    if torch.cuda.current_device() == x.device.index:
-        _lib.check(fn(*args, _lib.stream_ptr(x.device)), entry)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, _lib.stream_ptr(device))
     else:
-        with torch.cuda.device(x.device):
-            _lib.check(fn(*args, _lib.stream_ptr(x.device)), entry)
+        with torch.cuda.device(device):
+            rc = fn(*args, _lib.stream_ptr(device))
+    if rc < 0:
+        _lib.check(rc, entry)
 
 
-def _workspace(n_bytes, device):
-    return torch.empty(n_bytes, dtype=torch.uint8, device=device) if n_bytes else None
+def _address(t):
+    return 0 if t is None else t.data_ptr()
 
 
 # ----------------------------------------------------------------------------------------------------------- group norm
@@ -132,9 +134,9 @@ def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=None,
     if x.numel() == 0:
         return y
     ws_bytes = _lib.lib().sedmi_group_norm_workspace_bytes(n, frames, inner, c, num_groups, dtype)
-    ws = _workspace(ws_bytes, x.device)
-    _call(x, "sedmi_group_norm", _lib.ptr(x), _lib.ptr(weight), _lib.ptr(bias), _lib.ptr(lengths), _lib.ptr(y), n, frames,
-          inner, c, num_groups, float(eps), act, dtype, _lib.ptr(ws), ws_bytes)
+    ws = x.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+    _call(x.device, "sedmi_group_norm", x.data_ptr(), _address(weight), _address(bias), _address(lengths), y.data_ptr(), n,
+          frames, inner, c, num_groups, float(eps), act, dtype, _address(ws), ws_bytes)
     return y
 
 
@@ -165,12 +167,11 @@ def causal_conv1d(x, weight, bias=None, activation=None, state=None, lengths=Non
         state = _like(state, x, (n, k - 1, c), "state").contiguous()
     lengths = _lengths(lengths, n, x.device, "causal_conv1d")
     frames = x.shape[1]
-    y = torch.empty((n, frames, c), dtype=x.dtype, device=x.device)
-    last = torch.empty((n, k - 1, c), dtype=x.dtype, device=x.device) if return_state else None
+    y = x.new_empty((n, frames, c))
+    last = x.new_empty((n, k - 1, c)) if return_state else None
     if n and (frames or return_state):
-        _call(x, "sedmi_causal_conv1d", _lib.ptr(x), x.stride(0), x.stride(1), _lib.ptr(weight), _lib.ptr(bias),
-              _lib.ptr(lengths), _lib.ptr(state), _lib.ptr(last), _lib.ptr(y), n, frames, c, k, act, int(bool(reverse)),
-              dtype)
+        _call(x.device, "sedmi_causal_conv1d", x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(), _address(bias),
+              _address(lengths), _address(state), _address(last), y.data_ptr(), n, frames, c, k, act, bool(reverse), dtype)
     return (y, last) if return_state else y
 
 
@@ -187,10 +188,11 @@ def causal_conv1d_step(x, state, weight, bias=None, activation=None):
     _like(state, x, (n, k - 1, c), "state")
     if not state.is_contiguous():
         raise ValueError("causal_conv1d_step: the state is updated in place and has to be contiguous")
-    y = torch.empty((n, c), dtype=x.dtype, device=x.device)
+    y = x.new_empty((n, c))
     if n:
-        _call(x, "sedmi_causal_conv1d", _lib.ptr(x), x.stride(0), 0, _lib.ptr(weight), _lib.ptr(bias), None,
-              _lib.ptr(state), _lib.ptr(state), _lib.ptr(y), n, 1, c, k, act, 0, dtype)
+        at = state.data_ptr()
+        _call(x.device, "sedmi_causal_conv1d", x.data_ptr(), x.stride(0), 0, weight.data_ptr(), _address(bias), 0, at, at,
+              y.data_ptr(), n, 1, c, k, act, 0, dtype)
     return y
 
 
@@ -221,10 +223,6 @@ def _scan_arguments(x, dt, A, B, C, D, z, dt_bias, who):
             c, groups, m)
 
 
-def _address(t):
-    return None if t is None else t.data_ptr()
-
-
 def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=False, state=None, lengths=None,
                    reverse=False, return_state=False):
     """Selective state space scan of x [clips, frames, channels]:
@@ -248,19 +246,18 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fal
             raise TypeError(f"selective_scan: the state is float32, not {state.dtype}")
         state = _param(state, x, (n, c, m), "state")
     lengths = _lengths(lengths, n, x.device, "selective_scan")
-    y = torch.empty((n, frames, c), dtype=x.dtype, device=x.device)
-    last = torch.empty((n, c, m), dtype=torch.float32, device=x.device) if return_state else None
+    y = x.new_empty((n, frames, c))
+    last = x.new_empty((n, c, m), dtype=torch.float32) if return_state else None
     if not n or not (frames or return_state):
         return (y, last) if return_state else y
-    zs = (0, 0) if z is None else (z.stride(0), z.stride(1))
-    args = _lib.ScanArgs(x.data_ptr(), dt.data_ptr(), _address(z), B.data_ptr(), C.data_ptr(), A.data_ptr(), _address(D),
-                         _address(dt_bias), _address(lengths), _address(state), _address(last), y.data_ptr(),
-                         (x.stride(0), x.stride(1)), (dt.stride(0), dt.stride(1)), zs,
-                         B.stride()[:3], C.stride()[:3], n, frames, c, groups, m, dtype, int(bool(dt_softplus)),
-                         int(bool(reverse)))
+    args = _lib.pack_scan_args(x.data_ptr(), dt.data_ptr(), _address(z), B.data_ptr(), C.data_ptr(), A.data_ptr(),
+                               _address(D), _address(dt_bias), _address(lengths), _address(state), _address(last),
+                               y.data_ptr(), *x.stride()[:2], *dt.stride()[:2], *((0, 0) if z is None else z.stride()[:2]),
+                               *B.stride()[:3], *C.stride()[:3], n, frames, c, groups, m, dtype, bool(dt_softplus),
+                               bool(reverse))
     ws_bytes = _lib.lib().sedmi_selective_scan_workspace_bytes(n, frames, c, groups, m)
-    ws = _workspace(ws_bytes, x.device)
-    _call(x, "sedmi_selective_scan", args, _lib.ptr(ws), ws_bytes)
+    ws = x.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+    _call(x.device, "sedmi_selective_scan", args, _address(ws), ws_bytes)
     return (y, last) if return_state else y
 
 
@@ -277,13 +274,14 @@ def selective_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_softp
     if state.dtype != torch.float32 or not state.is_contiguous():
         raise ValueError("selective_step: the state is updated in place and has to be float32 and contiguous")
     _param(state, x, (n, c, m), "state")
-    y = torch.empty((n, c), dtype=x.dtype, device=x.device)
+    y = x.new_empty((n, c))
     if n:
-        zs = 0 if z is None else z.stride(0)
         at = state.data_ptr()
-        args = _lib.ScanArgs(x.data_ptr(), dt.data_ptr(), _address(z), B.data_ptr(), C.data_ptr(), A.data_ptr(),
-                             _address(D), _address(dt_bias), None, at, at, y.data_ptr(), (x.stride(0), 0),
-                             (dt.stride(0), 0), (zs, 0), (B.stride(0), 0, B.stride(1)), (C.stride(0), 0, C.stride(1)), n, 1,
-                             c, groups, m, dtype, int(bool(dt_softplus)), 0)
-        _call(x, "sedmi_selective_step", args)
+        b0, b1, _ = B.stride()
+        c0, c1, _ = C.stride()
+        args = _lib.pack_scan_args(x.data_ptr(), dt.data_ptr(), _address(z), B.data_ptr(), C.data_ptr(), A.data_ptr(),
+                                   _address(D), _address(dt_bias), 0, at, at, y.data_ptr(), x.stride(0), 0, dt.stride(0), 0,
+                                   0 if z is None else z.stride(0), 0, b0, 0, b1, c0, 0, c1, n, 1, c, groups, m, dtype,
+                                   bool(dt_softplus), 0)
+        _call(x.device, "sedmi_selective_step", args)
     return y

@@ -93,6 +93,8 @@ def test_scan_arguments_have_the_layout_of_the_header():
     from sound_event_detection_amd import _lib
     assert C.sizeof(_lib.ScanArgs) == 12 * 8 + 3 * 16 + 2 * 24 + 2 * 8 + 6 * 4
     assert _lib.ScanArgs.n_clips.offset == 12 * 8 + 3 * 16 + 2 * 24
+    a = _lib.ScanArgs(*range(1, 13), (13, 14), (15, 16), (17, 18), (19, 20, 21), (22, 23, 24), 25, 26, 27, 28, 29, 30, 1, 0)
+    assert bytes(a) == _lib.pack_scan_args(*range(1, 31), True, False)
 
 
 def test_cpu_tensors_are_refused():
