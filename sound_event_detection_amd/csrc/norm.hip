@@ -285,10 +285,14 @@ __global__ __launch_bounds__(1024) void norm_slab_kernel(const T *x, T *y, NormA
     Pack<T, V> in[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-        const int row = row_of(k);
+        const int row = row_of(k);                               // rows behind the last valid one repeat it, uncounted
         in[k] = Pack<T, V>::zero();
-        if (row < good) in[k] = column_of(k, row).load(px + static_cast<int64_t>(row) * a.channels);
+        if (good > 0) in[k] = column_of(k, row).load(px + static_cast<int64_t>(min(row, good - 1)) * a.channels);
     }
+    auto skip_of = [&](int k) __attribute__((always_inline)) {
+        const int row = row_of(k);
+        return row < good ? column_of(k, row).skip : V;
+    };
     // unpacked anew in each phase: kept as float32 between them, the rows would need twice the registers
     auto repack = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -308,7 +312,7 @@ __global__ __launch_bounds__(1024) void norm_slab_kernel(const T *x, T *y, NormA
     float sum = 0.0f, squares = 0.0f;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-        const int skip = column_of(k, row_of(k)).skip;
+        const int skip = skip_of(k);
 #pragma unroll
         for (int e = 0; e < V; ++e) sum += e >= skip ? in[k].get(e) : 0.0f;
     }
@@ -317,7 +321,7 @@ __global__ __launch_bounds__(1024) void norm_slab_kernel(const T *x, T *y, NormA
     repack();
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-        const int row = row_of(k), skip = row < good ? column_of(k, row).skip : V;
+        const int skip = skip_of(k);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             const float d = in[k].get(e) - mean;

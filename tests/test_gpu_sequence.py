@@ -300,6 +300,21 @@ def test_step(seq, n, c, groups, m, dtype):
     ref.check(held, end, end_bound, "state")
 
 
+@pytest.mark.parametrize("m", [3, 4, 18, 32])
+def test_step_of_many_streams(seq, m):
+    # enough streams that a quad of lanes takes four of them; their number is no multiple of four
+    n, c = 1027, 6
+    d, state = scan_inputs(55, n, None, c, m, 2, F16), rand(56, n, c, m)
+    one = {k: v if k in ("A", "D", "dt_bias") else v[:, None] for k, v in d.items()}
+    y, bound, end, end_bound = ref.selective_scan(**one, dt_softplus=True, state=state)
+    guard = torch.full((n + 8, c, m), 7.0, device="cuda")
+    held = guard[4:n + 4]
+    held.copy_(state)
+    ref.check(seq.selective_step(**on_gpu(d), state=held, dt_softplus=True), y[:, 0], bound[:, 0])
+    ref.check(held, end, end_bound, "state")
+    assert bool((guard[:4] == 7).all()) and bool((guard[n + 4:] == 7).all())
+
+
 def test_scan_far_values(seq):
     d = scan_inputs(51, 1, 40, 16, 4, 1, F32)
     d["dt"][0, 5] = 60.0                                           # softplus is the identity, the state is forgotten
