@@ -36,7 +36,7 @@ __device__ __forceinline__ void conv_run(const T *x, const T *state_in, T *state
     constexpr int V = kVec<T>, H = K - 1, U = 4, P = Pack<T, V>::kPer;
     const int ne = FULL ? V : a.channels - c0;
     auto load = [&](const T *p) { return load_pack<T, V>(p, FULL ? V : ne); };
-    auto store = [&](T *p, const Pack<T, V> &v) { store_pack<T, V>(p, v, FULL ? V : ne); };
+    auto store = [&](T *p, const Pack<T, V> &v) { stream_pack<T, V>(p, v, FULL ? V : ne); };
     // frame t of the processing order is row t, or row length - 1 - t of a reversed clip
     const int64_t turn = a.reverse && length > 0 ? length - 1 : 0;
     const int64_t sx = a.reverse ? -a.x_frame : a.x_frame, sy = a.reverse ? -a.channels : a.channels;
@@ -98,7 +98,8 @@ __device__ __forceinline__ void conv_run(const T *x, const T *state_in, T *state
             if (t >= 0) last[i] = load(px + t * sx);
         }
 #pragma unroll
-        for (int i = 0; i < H; ++i) store(state_out + state_at + static_cast<int64_t>(i) * a.channels, last[i]);
+        for (int i = 0; i < H; ++i)
+            store_pack<T, V>(state_out + state_at + static_cast<int64_t>(i) * a.channels, last[i], FULL ? V : ne);
     }
 
     T *to = py + t0 * sy;

@@ -45,7 +45,10 @@ struct Column {
     int at, skip, size;
     __device__ __forceinline__ Column(int j, int width) : at(TINY ? 0 : min(j * V, width - V)), skip(j * V - at), size(TINY ? width : V) {}
     __device__ __forceinline__ Pack<T, V> load(const T *p) const { return load_pack<T, V>(p + at, size); }
-    __device__ __forceinline__ void store(T *p, const Pack<T, V> &v) const { store_pack<T, V>(p + at, v, size); }
+    __device__ __forceinline__ void store(T *p, const Pack<T, V> &v, bool stream) const {
+        if (stream) stream_pack<T, V>(p + at, v, size);
+        else store_pack<T, V>(p + at, v, size);
+    }
     __device__ __forceinline__ bool counts(int e) const { return e >= skip && e < size; }
 };
 
@@ -250,9 +253,9 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(const T *x, T *y, 
             if (r + kUnroll < good) fetch(c, r + kUnroll);
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u)
-                if (r + u < good) c.store(y + from + (r + u) * stride, out[u]);
+                if (r + u < good) c.store(y + from + (r + u) * stride, out[u], true);
         }
-        for (int r = good; r < rows; ++r) c.store(y + from + r * stride, Pack<T, V>::zero());
+        for (int r = good; r < rows; ++r) c.store(y + from + r * stride, Pack<T, V>::zero(), true);
     }
 }
 
@@ -342,7 +345,8 @@ __global__ __launch_bounds__(1024) void norm_slab_kernel(const T *x, T *y, NormA
 #pragma unroll
         for (int e = 0; e < V; ++e)
             v[e] = activate(fmaf((in[k].get(e) - mean) * rstd, a.weight ? w.get(e) : 1.0f, b.get(e)), ACT < 0 ? a.act : ACT);
-        c.store(py + static_cast<int64_t>(row) * a.channels, row < good ? Pack<T, V>::from(v) : Pack<T, V>::zero());
+        c.store(py + static_cast<int64_t>(row) * a.channels, row < good ? Pack<T, V>::from(v) : Pack<T, V>::zero(),
+                a.per_group * sizeof(T) >= 64);
     }
 }
 

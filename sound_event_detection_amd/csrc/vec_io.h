@@ -87,6 +87,24 @@ __device__ __forceinline__ void store_pack(T *p, const Pack<T, V> &r, int n) {
     }
 }
 
+// The same for an output that the kernel does not touch again: a store that does not stay in L2 leaves it to the inputs
+// (us: convolution of 128 x 250 x 2048 bf16 61 -> 58, 16 x 1000 x 2047 33 -> 28; norm of 128 x 250 x 8 x 128 53 -> 47).  For
+// rows that are written in one go: with pieces of 32 bytes it takes longer (norm of 128 x 250 x 16 x 64 f32, 8 groups: 81 ->
+// 140).  The same on loads loses everywhere (norm of 64 x 250 x 1024, 32 groups: 18 -> 27), as neighbours share lines.
+template <typename T, int V>
+__device__ __forceinline__ void stream_pack(T *p, const Pack<T, V> &r, int n) {
+    constexpr int W = V / Pack<T, V>::kPer;
+    if (n >= V) {
+        using Words = uint32_t __attribute__((ext_vector_type(W), aligned(sizeof(T))));
+        Words w;
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = r.w[i];
+        __builtin_nontemporal_store(w, reinterpret_cast<Words *>(p));
+    } else {
+        store_pack<T, V>(p, r, n);
+    }
+}
+
 __device__ __forceinline__ float silu(float x) { return x * __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
 
 // Activation codes are SEDMI_ACT_* (sedmi.h); the code is uniform, the branch costs a scalar compare.
