@@ -29,7 +29,7 @@ struct ConvArgs {
     uint32_t blocks_per_clip;
 };
 
-// One lane's run.  FULL: all V channels exist; ACT: the activation, or -1 to look it up.
+// One lane's run.  FULL: all V channels exist; ACT: the activation.
 template <typename T, int K, bool FULL, int ACT>
 __device__ __forceinline__ void conv_run(const T *x, const T *state_in, T *state_out, T *y, const ConvArgs &a, int64_t clip,
                                          int segment, int c0, int64_t length) {
@@ -119,7 +119,7 @@ __device__ __forceinline__ void conv_run(const T *x, const T *state_in, T *state
                     float v = b[i * P + e];
 #pragma unroll
                     for (int k = 0; k < K; ++k) v = fmaf(w[(i * P + e) * K + k], f[u + k], v);
-                    s[u][e] = activate(v, ACT < 0 ? a.act : ACT);
+                    s[u][e] = activate<ACT>(v);
                 }
             }
 #pragma unroll

@@ -23,7 +23,6 @@ struct NormArgs {
     int64_t frames, inner, rows;         // rows = frames * inner
     int channels, groups, per_group;     // per_group = channels / groups
     float eps;
-    int act;
     // two-launch form
     int groups_per_block, column_blocks, chunks;
     int64_t rows_per_chunk;
@@ -247,7 +246,7 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(const T *x, T *y, 
                 float v[V];
 #pragma unroll
                 for (int e = 0; e < V; ++e)
-                    v[e] = activate(fmaf(in[u].get(e) - mean[e], scale[e], shift[e]), ACT < 0 ? a.act : ACT);
+                    v[e] = activate<ACT>(fmaf(in[u].get(e) - mean[e], scale[e], shift[e]));
                 out[u] = Pack<T, V>::from(v);
             }
             if (r + kUnroll < good) fetch(c, r + kUnroll);
@@ -344,7 +343,7 @@ __global__ __launch_bounds__(1024) void norm_slab_kernel(const T *x, T *y, NormA
         float v[V];
 #pragma unroll
         for (int e = 0; e < V; ++e)
-            v[e] = activate(fmaf((in[k].get(e) - mean) * rstd, a.weight ? w.get(e) : 1.0f, b.get(e)), ACT < 0 ? a.act : ACT);
+            v[e] = activate<ACT>(fmaf((in[k].get(e) - mean) * rstd, a.weight ? w.get(e) : 1.0f, b.get(e)));
         c.store(py + static_cast<int64_t>(row) * a.channels, row < good ? Pack<T, V>::from(v) : Pack<T, V>::zero(),
                 a.per_group * sizeof(T) >= 64);
     }
@@ -389,13 +388,13 @@ bool use_slab(int64_t clips, int64_t rows, int channels, int groups, int vec) {
 }
 
 template <typename T>
-void launch_slab(const T *x, T *y, NormArgs a, int64_t clips, hipStream_t st) {
+void launch_slab(const T *x, T *y, NormArgs a, int64_t clips, int activation, hipStream_t st) {
     a.vectors = static_cast<int>(sedmi::ceil_div(a.per_group, kVec<T>));
     a.per_row_inverse = a.vectors > 1 ? static_cast<uint32_t>((uint64_t{1} << 32) / a.vectors + 1) : 0;
     const int64_t vectors = a.rows * a.vectors;
     const int threads = vectors <= 512 ? 256 : vectors <= 1024 ? 512 : 1024;       // up to 2 vectors each, then up to 8
     const unsigned blocks = static_cast<unsigned>(clips * a.groups);
-    with_activation(a.act, [&](auto act) {
+    with_activation(activation, [&](auto act) {
         constexpr int kAct = decltype(act)::value;
         const int64_t each = sedmi::ceil_div(vectors, threads);
         if (each <= 1) norm_slab_kernel<T, 1, kAct><<<blocks, threads, 0, st>>>(x, y, a);
@@ -438,7 +437,7 @@ int sedmi_group_norm(const void *x, const float *weight, const float *bias, cons
     a.weight = weight, a.bias = bias, a.lengths = lengths;
     a.frames = frames, a.inner = inner, a.rows = frames * inner;
     a.channels = channels, a.groups = groups, a.per_group = channels / groups;
-    a.eps = eps, a.act = activation;
+    a.eps = eps;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const double items = static_cast<double>(n_clips) * a.rows * channels;
     const double es = dtype == SEDMI_DTYPE_F32 ? 4 : 2;
@@ -446,7 +445,7 @@ int sedmi_group_norm(const void *x, const float *weight, const float *bias, cons
         SEDMI_REQUIRE(n_clips * groups < (int64_t{1} << 31), "group_norm: too many workgroups");
         sedmi::ProfileScope scope("norm_slab_kernel", st, 8 * items, 2 * es * items);
         with_dtype(dtype, [&](auto t) -> int {
-            launch_slab(static_cast<const decltype(t) *>(x), static_cast<decltype(t) *>(y), a, n_clips, st);
+            launch_slab(static_cast<const decltype(t) *>(x), static_cast<decltype(t) *>(y), a, n_clips, activation, st);
             return SEDMI_OK;
         });
         SEDMI_CHECK_LAUNCH();
@@ -474,13 +473,11 @@ int sedmi_group_norm(const void *x, const float *weight, const float *bias, cons
         SEDMI_CHECK_LAUNCH();
         {
             sedmi::ProfileScope scope("norm_apply_kernel", st, 4 * items, 2 * es * items);
-            if (p.tiny) {
-                norm_apply_kernel<T, true, -1><<<grid, kThreads, 0, st>>>(px, py, a);
-            } else {
-                with_activation(activation, [&](auto act) {
-                    norm_apply_kernel<T, false, decltype(act)::value><<<grid, kThreads, 0, st>>>(px, py, a);
-                });
-            }
+            with_activation(activation, [&](auto act) {
+                constexpr int kAct = decltype(act)::value;
+                if (p.tiny) norm_apply_kernel<T, true, kAct><<<grid, kThreads, 0, st>>>(px, py, a);
+                else norm_apply_kernel<T, false, kAct><<<grid, kThreads, 0, st>>>(px, py, a);
+            });
         }
         SEDMI_CHECK_LAUNCH();
         return SEDMI_OK;
