@@ -262,7 +262,9 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(const T *x, T *y, 
 //
 // x is read once and held as it is in memory; mean, then the squares about it, then the output.  Workgroups of the groups
 // of one clip follow each other on one die (blocks are dealt to the 8 dies in turn), so lines that two groups share are
-// fetched into one L2.
+// fetched into one L2.  Groups of 32-byte rows (128 x 250 x 16 x 64 f32, 8 groups: 79 us, 3.3 TB/s) are bound by lines that
+// leave L2 before their neighbours come: more workgroups per compute unit (90 us) and a loop over groups that loads the next
+// one early (84 us) both lose.  Groups of 64-byte rows: 64 x 250 x 1024 bf16, 32 groups, 18 us.
 template <typename T, int N, int ACT>
 __global__ __launch_bounds__(1024) void norm_slab_kernel(const T *x, T *y, NormArgs a) {
     constexpr int V = kVec<T>;
@@ -332,14 +334,17 @@ __global__ __launch_bounds__(1024) void norm_slab_kernel(const T *x, T *y, NormA
     }
     const float rstd = 1.0f / sqrtf(total(squares, s_sum[1]) / items + a.eps);
     repack();
+    const bool one_column = threads % a.vectors == 0;            // all vectors of a thread lie in the same channels
+    Pack<float, V> w = Pack<float, V>::zero(), b = w;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         const int row = row_of(k);
-        if (row >= rows) continue;
         const auto c = column_of(k, row);
-        Pack<float, V> w, b = Pack<float, V>::zero();
-        if (a.weight) w = load_pack<float, V>(a.weight + c0 + c.at, V);
-        if (a.bias) b = load_pack<float, V>(a.bias + c0 + c.at, V);
+        if (k == 0 || !one_column) {
+            if (a.weight) w = load_pack<float, V>(a.weight + c0 + c.at, V);
+            if (a.bias) b = load_pack<float, V>(a.bias + c0 + c.at, V);
+        }
+        if (row >= rows) continue;
         float v[V];
 #pragma unroll
         for (int e = 0; e < V; ++e)
