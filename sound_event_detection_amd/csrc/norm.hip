@@ -262,9 +262,10 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(const T *x, T *y, 
 //
 // x is read once and held as it is in memory; mean, then the squares about it, then the output.  Workgroups of the groups
 // of one clip follow each other on one die (blocks are dealt to the 8 dies in turn), so lines that two groups share are
-// fetched into one L2.  Groups of 32-byte rows (128 x 250 x 16 x 64 f32, 8 groups: 79 us, 3.3 TB/s) are bound by lines that
-// leave L2 before their neighbours come: more workgroups per compute unit (90 us) and a loop over groups that loads the next
-// one early (84 us) both lose.  Groups of 64-byte rows: 64 x 250 x 1024 bf16, 32 groups, 18 us.
+// fetched into one L2: by the counters every byte crosses HBM once each way.  Measured: groups of 32-byte rows (128 x 250 x
+// 16 x 64 f32, 8 groups) 79 us, 3.3 TB/s; of 64-byte rows (64 x 250 x 1024 bf16, 32 groups) 18 us, 3.6 TB/s.  A workgroup
+// reads, sums and writes in turn; twice the workgroups per compute unit (90 us) and a loop that loads the next group early
+// (84 us) need more registers than there are and lose.
 template <typename T, int N, int ACT>
 __global__ __launch_bounds__(1024) void norm_slab_kernel(const T *x, T *y, NormArgs a) {
     constexpr int V = kVec<T>;
@@ -410,7 +411,7 @@ void launch_slab(const T *x, T *y, NormArgs a, int64_t clips, int activation, hi
 }
 
 bool norm_shape_ok(int64_t clips, int64_t frames, int64_t inner, int channels, int groups, int dtype) {
-    return frames >= 0 && inner > 0 && frames <= (int64_t{1} << 40) / inner &&
+    return frames >= 0 && inner > 0 && frames <= (int64_t{1} << 38) / inner &&
            sequence_shape_ok(clips, frames * inner, channels) && groups > 0 && channels % groups == 0 && dtype_ok(dtype);
 }
 

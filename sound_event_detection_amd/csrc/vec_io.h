@@ -143,10 +143,10 @@ inline bool dtype_ok(int dtype) {
     return dtype == SEDMI_DTYPE_F32 || dtype == SEDMI_DTYPE_F16 || dtype == SEDMI_DTYPE_BF16;
 }
 
-// Limits that keep every product of the extents below 2^63.
+// Limits that keep every offset, in bytes too, below 2^63.
 inline bool sequence_shape_ok(int64_t clips, int64_t frames, int64_t channels) {
-    return clips >= 0 && clips <= (int64_t{1} << 24) && frames >= 0 && frames <= (int64_t{1} << 40) / (channels > 0 ? channels : 1) &&
-           channels > 0 && channels <= (1 << 24);
+    return clips >= 0 && clips <= (int64_t{1} << 22) && channels > 0 && channels <= (1 << 24) && frames >= 0 &&
+           frames <= (int64_t{1} << 38) / channels;
 }
 
 inline bool overlap(const void *p, const void *q, size_t bytes) {

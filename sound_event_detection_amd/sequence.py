@@ -15,12 +15,14 @@ there is no backward and no CPU path.
 
 Common to all: activations are float32, float16 or bfloat16, one type per call, and the results have that type;
 parameters are taken as float32 (others are converted in the call), sums, statistics and the scan's states are
-float32, each result is rounded once.  The channel dimension has to be adjacent in memory (a tensor where it is not is copied), the other
-strides are free, so slices of a wider projection are read in place.  ``lengths`` gives the valid frames of each clip
-(an int tensor or a sequence, values outside 0 .. frames are taken as the nearer end): frames behind them are never
-read and come out as zeros.  ``reverse=True`` runs from a clip's last valid frame to its first, the second direction
-of a bidirectional layer.  Nothing is kept between calls and nothing waits for the GPU; all work goes to the current
-stream of the tensors' device.
+float32, each result is rounded once.  The channel dimension has to be adjacent in memory (a tensor where it is not is
+copied), the other strides are free, so slices of a wider projection are read in place (``group_norm`` copies what is
+not contiguous).  ``lengths`` gives the valid frames of each clip (an int tensor or a sequence, values outside
+0 .. frames are taken as the nearer end): frames behind them are never read and come out as zeros.  An int64 tensor on
+the device is used as it is; anything else is copied there first, which waits for the copy and cannot be captured into
+a graph.  ``reverse=True`` runs from a clip's last valid frame to its first, the second direction of a bidirectional
+layer.  Nothing is kept between calls; all work goes to the current stream of the tensors' device, and apart from that
+copy nothing waits for it.
 """
 from __future__ import annotations
 
