@@ -82,6 +82,8 @@ def _lengths(lengths, n, device, who):
     if lengths is None:
         return None
     t = lengths if torch.is_tensor(lengths) else torch.as_tensor(lengths)
+    if t.dtype is torch.int64 and t.is_cuda and t.shape == (n,) and t.device == device:
+        return t.contiguous()
     if t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{who}: lengths needs one entry per clip ({n}), got shape {tuple(t.shape)}")
     if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
@@ -199,30 +201,26 @@ def causal_conv1d_step(x, state, weight, bias=None, activation=None):
 
 
 # ------------------------------------------------------------------------------------------------------- selective scan
-def _pair(t, shape, x, what):
-    """B or C with its group dimension: [.., states] stands for one group."""
-    if t.dim() == len(shape) - 1:
-        t = t.unsqueeze(-2)
-    if t.dim() != len(shape):
-        raise ValueError(f"{what}: expected {len(shape)} dimensions (or {len(shape) - 1} for one group), got {tuple(t.shape)}")
-    return _like(t, x, (*shape[:-2], t.shape[-2], shape[-1]), what)
-
-
 def _scan_arguments(x, dt, A, B, C, D, z, dt_bias, who):
-    c = x.shape[-1]
+    shape = x.shape
+    c, lead = shape[-1], shape[:-1]
     if A.dim() != 2 or A.shape[0] != c or not 1 <= A.shape[1] <= MAX_STATES:
         raise ValueError(f"{who}: expected A [{c}, 1 .. {MAX_STATES}], got {tuple(A.shape)}")
     m = A.shape[1]
-    lead = x.shape[:-1]
     x = x if x.stride(-1) == 1 or c == 1 else x.contiguous()
-    dt = _like(dt, x, x.shape, "dt")
-    z = None if z is None else _like(z, x, x.shape, "z")
-    B, C = _pair(B, (*lead, 0, m), x, "B"), _pair(C, (*lead, 0, m), x, "C")
-    groups = B.shape[-2]
-    if C.shape[-2] != groups or groups < 1 or c % groups:
-        raise ValueError(f"{who}: {c} channels, B with {groups} and C with {C.shape[-2]} groups do not go together")
-    return (x, dt, z, B, C, _param(A, x, (c, m), "A"), _param(D, x, (c,), "D"), _param(dt_bias, x, (c,), "dt_bias"),
-            c, groups, m)
+    dt = _like(dt, x, shape, "dt")
+    z = None if z is None else _like(z, x, shape, "z")
+    if B.dim() == len(shape):                      # [.., states] stands for one group
+        B = B.unsqueeze(-2)
+    if C.dim() == len(shape):
+        C = C.unsqueeze(-2)
+    groups = B.shape[-2] if B.dim() == len(shape) + 1 else 0
+    if groups < 1 or c % groups:
+        raise ValueError(f"{who}: {c} channels and B {tuple(B.shape)}: expected {tuple(lead)} + [groups, {m}] or + [{m}], the "
+                         "groups dividing the channels")
+    both = (*lead, groups, m)
+    return (x, dt, z, _like(B, x, both, "B"), _like(C, x, both, "C"), _param(A, x, (c, m), "A"), _param(D, x, (c,), "D"),
+            _param(dt_bias, x, (c,), "dt_bias"), c, groups, m)
 
 
 def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=False, state=None, lengths=None,
