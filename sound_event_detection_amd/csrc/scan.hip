@@ -18,6 +18,10 @@ constexpr int kThreads = 256;
 // Four lanes share a channel and hold a quarter of its N states each, in registers, from the first frame to the
 // last; a workgroup owns 64 channels of one clip.  Tiles of kTile frames go through LDS: there d and d*x are formed
 // once per (frame, channel) instead of once per lane, and the four lanes of a channel read them as broadcasts.
+//
+// The vector unit bounds it: one exponential and three products or sums per (frame, channel, state), 41 operations per
+// (frame, channel) around them.  64 x 250 x 1024 x 16 bf16: 72 us (135 MB, 26 us at the rate of a copy), of which the vector
+// unit issues for 61; 2 x 6000 x 1024 x 16 f16 in 32 runs: 103 us, 43 of them in the first pass.
 constexpr int kChannels = 64;            // per workgroup
 constexpr int kTile = 32;                // frames staged at a time
 constexpr int kYStride = kChannels + 16; // of the y tile: rows a wave writes together lie in different banks
@@ -82,7 +86,7 @@ using F4 = __attribute__((ext_vector_type(4))) float;
 // NP >= 4 states per lane those are n = 16 k + 4 q + i, k < NP / 4, i < 4.  That is the layout of sixteen 4 x 4 blocks of
 // the matrix instruction v_mfma_f32_4x4x1 (row i in register i, column = lane & 3), so d x B^T, an outer product of 4
 // channels and 4 states per block, is added to exp(d A) h by the matrix unit while the vector unit, which bounds this
-// kernel, forms the next exponents.  Up to 8 states (NP < 4) a lane holds n = q NP + i and adds them itself.
+// kernel, forms the next exponents (64 x 250 x 1024 x 16: 83 us without, 77 with, all else equal).  Up to 8 states (NP < 4) a lane holds n = q NP + i and adds them itself.
 //
 // Two workgroups per compute unit at least: with at most 256 registers the compiler keeps the matrix instruction's
 // accumulators in ordinary registers, which saves eight moves per frame.
@@ -373,8 +377,8 @@ __device__ __forceinline__ float quad_lane(float v) {
 // does the work per channel (step size, gate, output) of one stream.
 //
 // WHOLE (at least 4 states): every 16-byte piece is loaded whole, the last one moved back over its neighbour's states, and
-// lanes past it load it for nothing, so no branch holds up a load (256 streams x 2048 x 16: 13 us, 27 with a branch for
-// each piece).  Elements in two pieces get the same value from both; every load of a wave comes before its stores.
+// lanes past it load it for nothing, so no branch holds up a load (256 streams x 2048 x 16 bf16: 13 us, 5.4 TB/s; 27 with a
+// branch for each piece).  Elements in two pieces get the same value from both; every load of a wave comes before its stores.
 template <typename T, int NI, int M, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void selective_step_kernel(ScanArgs a, float *state, int64_t clips) {
     static_assert(M == 1 || M == 4, "one stream, or one per lane of a quad");
