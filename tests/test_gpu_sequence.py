@@ -424,6 +424,52 @@ def test_a_layer_on_another_stream_and_in_a_graph(seq):
             assert torch.equal(out, want)
 
 
+def test_captured_steps_move_their_states_on_at_every_replay(seq):
+    c, m, k, n = 40, 16, 4, 5
+    w = layer_weights(c, m, k)
+
+    def step(x, conv_state, scan_state):
+        v = seq.causal_conv1d_step(x, conv_state, w["conv_w"], w["conv_b"], "silu")
+        bc = v @ w["to_bc"]
+        return seq.selective_step(v, v @ w["to_dt"], w["A"], bc[:, :m], bc[:, m:], scan_state, D=w["D"], z=x,
+                                  dt_bias=w["dt_bias"], dt_softplus=True)
+
+    def fresh():
+        return torch.zeros(n, k - 1, c, device="cuda"), torch.zeros(n, c, m, device="cuda")
+
+    held, states, eager = torch.zeros(n, c, device="cuda"), fresh(), fresh()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(held, *fresh())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(held, *states)
+    for i in range(6):
+        x = rand(100 + i, n, c).cuda()
+        want = step(x, *eager)
+        held.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert torch.equal(states[0], eager[0]) and torch.equal(states[1], eager[1])
+
+
+def test_kernels_report_to_the_profiler(seq):
+    from sound_event_detection_amd import _lib
+    d = on_gpu(scan_inputs(97, 1, 300, 16, 4, 1, F32))
+    _lib.profile_enable(True)
+    try:
+        seq.group_norm(d["x"], 2)
+        seq.causal_conv1d(d["x"], torch.zeros(16, 4, device="cuda"))
+        seq.selective_scan(**d, dt_softplus=True)
+        names = {k["name"] for k in _lib.profile_collect()}
+    finally:
+        _lib.profile_enable(False)
+    assert {"norm_slab_kernel", "causal_conv_kernel", "selective_scan_end_kernel", "selective_scan_kernel"} <= names
+
+
 def test_the_same_call_gives_the_same_bits(seq):
     d = on_gpu(scan_inputs(80, 1, 1500, 40, 16, 1, BF16))
     x = rand(81, 2, 500, 16, 64).cuda()
