@@ -16,15 +16,14 @@ constexpr int kThreads = 256;
 //     y_t[c] = (sum_n C_t[g(c), n] h_t[c, n] + D[c] x_t[c]) * silu(z_t[c])
 //
 // Four lanes share a channel and hold a quarter of its N states each, in registers, from the first frame to the
-// last; a workgroup owns 64 channels of one clip.  Tiles of kTile frames go through LDS: there d and d*x are formed
+// last; a workgroup owns 64 (or 16) channels of one clip.  Tiles of kTile frames go through LDS: there d and d*x are formed
 // once per (frame, channel) instead of once per lane, and the four lanes of a channel read them as broadcasts.
 //
 // The vector unit bounds it: one exponential and three products or sums per (frame, channel, state), 41 operations per
 // (frame, channel) around them.  64 x 250 x 1024 x 16 bf16: 72 us (135 MB, 26 us at the rate of a copy), of which the vector
 // unit issues for 61; 2 x 6000 x 1024 x 16 f16 in 32 runs: 103 us, 43 of them in the first pass.
-constexpr int kChannels = 64;            // per workgroup
 constexpr int kTile = 32;                // frames staged at a time
-constexpr int kYStride = kChannels + 16; // of the y tile: rows a wave writes together lie in different banks
+constexpr int kStepChannels = 64;        // per workgroup of the single-frame form
 
 struct ScanArgs {
     const void *x, *dt, *B, *C, *z;
@@ -88,10 +87,14 @@ using F4 = __attribute__((ext_vector_type(4))) float;
 // channels and 4 states per block, is added to exp(d A) h by the matrix unit while the vector unit, which bounds this
 // kernel, forms the next exponents (64 x 250 x 1024 x 16: 83 us without, 77 with, all else equal).  Up to 8 states (NP < 4) a lane holds n = q NP + i and adds them itself.
 //
-// Two workgroups per compute unit at least: with at most 256 registers the compiler keeps the matrix instruction's
+// Two waves per SIMD at least: with at most 256 registers the compiler keeps the matrix instruction's
 // accumulators in ordinary registers, which saves eight moves per frame.
-template <typename T, int NP, bool END>
-__global__ __launch_bounds__(kThreads, 2) void selective_scan_kernel(ScanArgs a) {
+//
+// WAVES: 4, or 1 for groups of up to 32 channels with up to 16 states, whose workgroups of 64 would leave half of their lanes idle or more.
+template <typename T, int NP, bool END, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void selective_scan_kernel(ScanArgs a) {
+    constexpr int kThreads = 64 * WAVES, kChannels = 16 * WAVES;
+    constexpr int kYStride = kChannels + 16;                     // rows of y that a wave writes together: different banks
     constexpr int N4 = 4 * NP;                                   // states staged per frame, zero beyond a.states
     constexpr bool kMatrix = NP >= 4;
     constexpr int kBRows = kThreads / N4 < kTile ? kThreads / N4 : kTile;    // rows of B that the workgroup loads at a time
@@ -120,7 +123,7 @@ __global__ __launch_bounds__(kThreads, 2) void selective_scan_kernel(ScanArgs a)
     // lane loads the pair before it and takes the second; lanes beside the last channel load the last pair for nothing.
     const int64_t turn = a.reverse && length > 0 ? length - 1 : 0;
     const int dir = a.reverse ? -1 : 1;
-    const int sc = (tid & 31) * 2, sr = tid >> 5;
+    const int sc = tid % (kChannels / 2) * 2, sr = tid / (kChannels / 2);
     const int sn = min(2, width - sc), pair = max(0, min(sc, width - 2));
     const bool second = sc - pair == 1 && width > 1;
     const int64_t row0 = turn + dir * t0;
@@ -387,8 +390,8 @@ __global__ __launch_bounds__(kThreads) void selective_step_kernel(ScanArgs a, fl
     const int64_t clip0 = blockIdx.x / per_clip * static_cast<int64_t>(M);
     const int cb = blockIdx.x % per_clip;
     const int group = cb / a.blocks_per_group;
-    const int first = (cb - group * a.blocks_per_group) * kChannels;
-    if (ch >= min(kChannels, a.per_group - first)) return;       // all four lanes of a channel leave together
+    const int first = (cb - group * a.blocks_per_group) * kStepChannels;
+    if (ch >= min(kStepChannels, a.per_group - first)) return;       // all four lanes of a channel leave together
     const int c = group * a.per_group + first + ch;
     const float *pa = a.A + static_cast<int64_t>(c) * a.states;
     Pack<float, 4> hs[M][NI], as[NI];
@@ -450,9 +453,14 @@ __global__ __launch_bounds__(kThreads) void selective_step_kernel(ScanArgs a, fl
 
 constexpr int kMaxStates = 128;
 
-int64_t scan_blocks(int channels, int groups) {
-    return static_cast<int64_t>(groups) * sedmi::ceil_div(channels / groups, kChannels);
+int64_t blocks_of(int channels, int groups, int width) {
+    return static_cast<int64_t>(groups) * sedmi::ceil_div(channels / groups, width);
 }
+
+// Waves of a scan's workgroup, 16 channels each.  Four against one for narrow groups (us): 64 clips x 1165 frames x 29
+// channels x 16 states 52.6 / 41.5, 128 x 250 x 4 groups of 16 45.5 / 36.4, 47 x 138 x 4 groups of 5 27.7 / 20.9; with 32
+// states, whose rows take a wave alone twice as long to stage, 1 x 74 x 4 groups of 14 20.8 / 22.1.
+int scan_waves(int channels, int groups, int states) { return channels / groups <= 32 && states <= 16 ? 1 : 4; }
 
 int64_t scan_run(int64_t frames, int splits) {
     return sedmi::ceil_div(sedmi::ceil_div(std::max<int64_t>(frames, 1), splits), kTile) * kTile;
@@ -460,13 +468,14 @@ int64_t scan_run(int64_t frames, int splits) {
 
 // Runs of the time axis.  Splitting costs a second pass over all but the last run (0.6 of the scan itself), a launch and
 // the joining, so time is only split where workgroups are missing, down to one tile per run and up to four workgroups per
-// compute unit.  Measured, whole against split (N = 16, us): 16 workgroups x 250 frames 30 / 18, 10 x 1000 103 / 22,
+// compute unit (16 waves).  Measured, whole against split (N = 16, us): 16 workgroups of 4 waves x 250 frames 30 / 18, 10 x 1000 103 / 22,
 // 64 x 250 30 / 19, 32 x 6000 605 / 107; 256 x 250 32 / 39, 384 x 1000 152 / 169; 8 x 64 10 / 12.  More than 64 runs
 // lose to the joining (4 x 6000: 64 runs 41, 94 runs 47).
-int scan_splits(int64_t clips, int64_t frames, int channels, int groups) {
-    const int64_t have = std::max<int64_t>(1, clips * scan_blocks(channels, groups));
-    if (have >= 192 || frames < 128) return 1;
-    const int64_t splits = std::min<int64_t>({sedmi::ceil_div(1024, have), frames / kTile, 64});
+int scan_splits(int64_t clips, int64_t frames, int channels, int groups, int states) {
+    const int waves = scan_waves(channels, groups, states);
+    const int64_t have = std::max<int64_t>(1, clips * blocks_of(channels, groups, 16 * waves) * waves);
+    if (have >= 768 || frames < 128) return 1;
+    const int64_t splits = std::min<int64_t>({sedmi::ceil_div(4096, have), frames / kTile, 64});
     return static_cast<int>(sedmi::ceil_div(frames, scan_run(frames, static_cast<int>(splits))));
 }
 
@@ -497,19 +506,24 @@ ScanArgs scan_args(const sedmi_scan_args *p) {
     a.c_clip = p->C_stride[0], a.c_frame = p->C_stride[1], a.c_group = p->C_stride[2];
     a.frames = p->frames, a.channels = p->channels, a.states = p->states, a.groups = p->groups;
     a.per_group = p->channels / p->groups;
-    a.blocks_per_group = static_cast<int>(sedmi::ceil_div(a.per_group, kChannels));
     a.softplus = p->dt_softplus, a.reverse = p->reverse;
     return a;
 }
 
 template <typename T, bool END>
-void launch_scan(int states, unsigned blocks, hipStream_t st, const ScanArgs &a) {
-    if (states <= 4) selective_scan_kernel<T, 1, END><<<blocks, kThreads, 0, st>>>(a);
-    else if (states <= 8) selective_scan_kernel<T, 2, END><<<blocks, kThreads, 0, st>>>(a);
-    else if (states <= 16) selective_scan_kernel<T, 4, END><<<blocks, kThreads, 0, st>>>(a);
-    else if (states <= 32) selective_scan_kernel<T, 8, END><<<blocks, kThreads, 0, st>>>(a);
-    else if (states <= 64) selective_scan_kernel<T, 16, END><<<blocks, kThreads, 0, st>>>(a);
-    else selective_scan_kernel<T, 32, END><<<blocks, kThreads, 0, st>>>(a);
+void launch_scan(int states, int waves, unsigned blocks, hipStream_t st, const ScanArgs &a) {
+    if (waves == 1) {
+        if (states <= 4) selective_scan_kernel<T, 1, END, 1><<<blocks, 64, 0, st>>>(a);
+        else if (states <= 8) selective_scan_kernel<T, 2, END, 1><<<blocks, 64, 0, st>>>(a);
+        else selective_scan_kernel<T, 4, END, 1><<<blocks, 64, 0, st>>>(a);
+    } else {
+        if (states <= 4) selective_scan_kernel<T, 1, END, 4><<<blocks, 256, 0, st>>>(a);
+        else if (states <= 8) selective_scan_kernel<T, 2, END, 4><<<blocks, 256, 0, st>>>(a);
+        else if (states <= 16) selective_scan_kernel<T, 4, END, 4><<<blocks, 256, 0, st>>>(a);
+        else if (states <= 32) selective_scan_kernel<T, 8, END, 4><<<blocks, 256, 0, st>>>(a);
+        else if (states <= 64) selective_scan_kernel<T, 16, END, 4><<<blocks, 256, 0, st>>>(a);
+        else selective_scan_kernel<T, 32, END, 4><<<blocks, 256, 0, st>>>(a);
+    }
 }
 
 template <typename T, int M>
@@ -529,7 +543,7 @@ extern "C" {
 
 size_t sedmi_selective_scan_workspace_bytes(int64_t n_clips, int64_t frames, int channels, int groups, int states) {
     if (!scan_shape_ok(n_clips, frames, channels, groups, states)) return 0;
-    const int splits = scan_splits(n_clips, frames, channels, groups);
+    const int splits = scan_splits(n_clips, frames, channels, groups, states);
     return static_cast<size_t>(n_clips) * (splits - 1) * channels * (states + 1) * sizeof(float);
 }
 
@@ -541,14 +555,16 @@ int sedmi_selective_scan(const sedmi_scan_args *p, void *ws, size_t ws_bytes, vo
     SEDMI_REQUIRE(p->A != nullptr, "selective_scan: null A");
     SEDMI_REQUIRE(p->frames == 0 || (p->x && p->dt && p->B && p->C && p->y), "selective_scan: null x, dt, B, C or y");
     ScanArgs a = scan_args(p);
-    a.splits = scan_splits(p->n_clips, p->frames, p->channels, p->groups);
+    const int waves = scan_waves(p->channels, p->groups, p->states);
+    a.blocks_per_group = static_cast<int>(sedmi::ceil_div(a.per_group, 16 * waves));
+    a.splits = scan_splits(p->n_clips, p->frames, p->channels, p->groups, p->states);
     a.run = scan_run(p->frames, a.splits);
     const size_t need = sedmi_selective_scan_workspace_bytes(p->n_clips, p->frames, p->channels, p->groups, p->states);
     if (need > 0 && (ws == nullptr || ws_bytes < need))
         return sedmi::set_error(SEDMI_ENOMEM, "selective_scan: workspace of %zu bytes, %zu needed", ws_bytes, need);
     a.end_state = static_cast<float *>(ws);
     a.end_step = a.end_state + static_cast<size_t>(p->n_clips) * (a.splits - 1) * p->channels * p->states;
-    const int64_t blocks = p->n_clips * scan_blocks(p->channels, p->groups);
+    const int64_t blocks = p->n_clips * blocks_of(p->channels, p->groups, 16 * waves);
     SEDMI_REQUIRE(blocks * a.splits < (int64_t{1} << 31), "selective_scan: too many workgroups");
     hipStream_t st = static_cast<hipStream_t>(stream);
     const double items = static_cast<double>(p->n_clips) * p->frames * p->channels;
@@ -557,12 +573,12 @@ int sedmi_selective_scan(const sedmi_scan_args *p, void *ws, size_t ws_bytes, vo
         using T = decltype(t);
         if (a.splits > 1) {
             sedmi::ProfileScope scope("selective_scan_end_kernel", st, 5 * items * p->states, 2 * es * items);
-            launch_scan<T, true>(p->states, static_cast<unsigned>(blocks * (a.splits - 1)), st, a);
+            launch_scan<T, true>(p->states, waves, static_cast<unsigned>(blocks * (a.splits - 1)), st, a);
         }
         SEDMI_CHECK_LAUNCH();
         {
             sedmi::ProfileScope scope("selective_scan_kernel", st, 7 * items * p->states, (p->z ? 4 : 3) * es * items);
-            launch_scan<T, false>(p->states, static_cast<unsigned>(blocks * a.splits), st, a);
+            launch_scan<T, false>(p->states, waves, static_cast<unsigned>(blocks * a.splits), st, a);
         }
         SEDMI_CHECK_LAUNCH();
         return SEDMI_OK;
@@ -576,8 +592,9 @@ int sedmi_selective_step(const sedmi_scan_args *p, void *stream) {
     SEDMI_REQUIRE(p->state_in == p->state_out, "selective_step: the state is updated in place (state_in == state_out)");
     if (p->n_clips == 0) return SEDMI_OK;
     SEDMI_REQUIRE(p->A && p->x && p->dt && p->B && p->C && p->y && p->state_out, "selective_step: null pointer");
-    const ScanArgs a = scan_args(p);
-    const int64_t per_clip = scan_blocks(p->channels, p->groups), blocks = p->n_clips * per_clip;
+    ScanArgs a = scan_args(p);
+    a.blocks_per_group = static_cast<int>(sedmi::ceil_div(a.per_group, kStepChannels));
+    const int64_t per_clip = blocks_of(p->channels, p->groups, kStepChannels), blocks = p->n_clips * per_clip;
     SEDMI_REQUIRE(blocks < (int64_t{1} << 31), "selective_step: too many workgroups");
     hipStream_t st = static_cast<hipStream_t>(stream);
     const double items = static_cast<double>(p->n_clips) * p->channels;
