@@ -24,7 +24,7 @@ struct NormArgs {
     int channels, groups, per_group;     // per_group = channels / groups
     float eps;
     // two-launch form
-    int groups_per_block, column_blocks, chunks;
+    int groups_per_block, wider_blocks, column_blocks, chunks;  // the first wider_blocks have one group more
     int64_t rows_per_chunk;
     // one-launch form
     int vectors;                         // of a row of the group
@@ -67,8 +67,8 @@ __global__ __launch_bounds__(kThreads) void norm_stats_kernel(const T *x, NormAr
     const int64_t rest = blockIdx.x / a.column_blocks;
     const int chunk = static_cast<int>(rest % a.chunks);
     const int64_t clip = rest / a.chunks;
-    const int g0 = block * a.groups_per_block;
-    const int ng = min(a.groups_per_block, a.groups - g0);
+    const int g0 = block * a.groups_per_block + min(block, a.wider_blocks);
+    const int ng = a.groups_per_block + (block < a.wider_blocks);
     const int width = ng * a.per_group;                         // channels of this block
     const int nv = (width + V - 1) / V;
     const int64_t valid = clamp_length(a.lengths, clip, a.frames) * a.inner;
@@ -178,8 +178,8 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(const T *x, T *y, 
     const int64_t rest = blockIdx.x / a.column_blocks;
     const int chunk = static_cast<int>(rest % a.chunks);
     const int64_t clip = rest / a.chunks;
-    const int g0 = block * a.groups_per_block;
-    const int ng = min(a.groups_per_block, a.groups - g0);
+    const int g0 = block * a.groups_per_block + min(block, a.wider_blocks);
+    const int ng = a.groups_per_block + (block < a.wider_blocks);
     const int width = ng * a.per_group;
     const int nv = (width + V - 1) / V;
     const int64_t valid = clamp_length(a.lengths, clip, a.frames) * a.inner;
@@ -358,20 +358,23 @@ __global__ __launch_bounds__(1024) void norm_slab_kernel(const T *x, T *y, NormA
 
 // Row chunks and column blocks of the two-launch form.
 struct NormPlan {
-    int groups_per_block, column_blocks, chunks;
+    int groups_per_block, wider_blocks, column_blocks, chunks;
     int64_t rows_per_chunk;
-    bool tiny;                           // the narrowest block has fewer channels than a vector
+    bool tiny;                           // fewer channels than a vector
 };
 
 NormPlan norm_plan(int64_t clips, int64_t rows, int channels, int groups, int vec) {
     NormPlan p;
     const int per_group = channels / groups;
-    p.groups_per_block = std::max(1, std::min(groups, kThreads * vec / per_group));
-    p.column_blocks = static_cast<int>(sedmi::ceil_div(groups, p.groups_per_block));
-    p.groups_per_block = static_cast<int>(sedmi::ceil_div(groups, p.column_blocks));         // blocks of nearly one width
-    p.column_blocks = static_cast<int>(sedmi::ceil_div(groups, p.groups_per_block));
-    p.tiny = (groups - (p.column_blocks - 1) * p.groups_per_block) * per_group < vec;
-    const int nv = std::min<int64_t>(kThreads, sedmi::ceil_div(static_cast<int64_t>(p.groups_per_block) * per_group, vec));
+    // Blocks of at most kThreads vectors, the groups dealt out evenly: more than half of the widest possible block goes to
+    // each of several, so none is narrower than a vector.
+    const int fit = std::max(1, std::min(groups, kThreads * vec / per_group));
+    p.column_blocks = static_cast<int>(sedmi::ceil_div(groups, fit));
+    p.groups_per_block = groups / p.column_blocks;
+    p.wider_blocks = groups % p.column_blocks;
+    p.tiny = channels < vec;
+    const int widest = p.groups_per_block + (p.wider_blocks > 0);
+    const int nv = std::min<int64_t>(kThreads, sedmi::ceil_div(static_cast<int64_t>(widest) * per_group, vec));
     const int64_t rp = kThreads / nv;
     // Every workgroup joins statistics, so few: two per compute unit (128 x 250 x 8 x 128 with 32 groups, bf16: 512 53 us,
     // 1024 57, 2048 74), and no less than kUnroll rows for each of its threads.
@@ -459,7 +462,7 @@ int sedmi_group_norm(const void *x, const float *weight, const float *bias, cons
         return SEDMI_OK;
     }
     const NormPlan p = norm_plan(n_clips, a.rows, channels, groups, dtype_vec(dtype));
-    a.groups_per_block = p.groups_per_block, a.column_blocks = p.column_blocks;
+    a.groups_per_block = p.groups_per_block, a.wider_blocks = p.wider_blocks, a.column_blocks = p.column_blocks;
     a.chunks = p.chunks, a.rows_per_chunk = p.rows_per_chunk;
     const int64_t blocks = n_clips * p.chunks * p.column_blocks;
     SEDMI_REQUIRE(blocks < (int64_t{1} << 31), "group_norm: too many workgroups (%lld)", static_cast<long long>(blocks));
