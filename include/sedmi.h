@@ -436,7 +436,8 @@ int sedmi_confusion_counts(const float *p, const float *labels, int64_t n_rows, 
  * lengths: device int64 [n_clips] or NULL (= all frames).  Frames at and behind
  * lengths[i] (clamped to 0 .. frames) are never read, and their outputs are 0.
  * Limits (SEDMI_EINVAL beyond them): 2^22 clips, 2^24 channels, 2^38 elements
- * per clip, 2^31 workgroups.  No buffer is needed beyond the call's own work on
+ * per clip; one clip's workgroups must fit a launch (fewer than 2^32 threads),
+ * more clips than that take several.  No buffer is needed beyond the call's own work on
  * `stream`; calls on different streams need workspaces of their own.
  * ------------------------------------------------------------------------ */
 #define SEDMI_DTYPE_F32   0

@@ -166,16 +166,14 @@ __global__ __launch_bounds__(kThreads) void causal_conv_kernel(const T *x, const
 }
 
 template <typename T, int K>
-void launch_conv(unsigned blocks, hipStream_t st, const void *x, const void *si, void *so, void *y, const ConvArgs &a) {
+void launch_conv(unsigned blocks, hipStream_t st, const T *x, const T *si, T *so, T *y, const ConvArgs &a) {
     with_activation(a.act, [&](auto act) {
-        causal_conv_kernel<T, K, decltype(act)::value><<<blocks, kThreads, 0, st>>>(
-            static_cast<const T *>(x), static_cast<const T *>(si), static_cast<T *>(so), static_cast<T *>(y), a);
+        causal_conv_kernel<T, K, decltype(act)::value><<<blocks, kThreads, 0, st>>>(x, si, so, y, a);
     });
 }
 
 template <typename T>
-int launch_conv(int width, unsigned blocks, hipStream_t st, const void *x, const void *si, void *so, void *y,
-                const ConvArgs &a) {
+void launch_conv(int width, unsigned blocks, hipStream_t st, const T *x, const T *si, T *so, T *y, const ConvArgs &a) {
     switch (width) {
         case 1: launch_conv<T, 1>(blocks, st, x, si, so, y, a); break;
         case 2: launch_conv<T, 2>(blocks, st, x, si, so, y, a); break;
@@ -186,8 +184,6 @@ int launch_conv(int width, unsigned blocks, hipStream_t st, const void *x, const
         case 7: launch_conv<T, 7>(blocks, st, x, si, so, y, a); break;
         default: launch_conv<T, 8>(blocks, st, x, si, so, y, a); break;
     }
-    SEDMI_CHECK_LAUNCH();
-    return SEDMI_OK;
 }
 
 }  // namespace
@@ -222,15 +218,25 @@ int sedmi_causal_conv1d(const void *x, int64_t x_stride_clip, int64_t x_stride_f
     while (a.rows < 32 && n_clips * sedmi::ceil_div(frames, a.rows) * a.vectors > 262144) a.rows *= 2;
     a.in_place = state_in != nullptr && state_in == state_out;
     const int64_t segments = std::max<int64_t>(1, sedmi::ceil_div(frames, a.rows));      // no frames: the state alone
-    const int64_t per_clip = sedmi::ceil_div(segments * a.vectors, kThreads), blocks = per_clip * n_clips;
-    SEDMI_REQUIRE(segments < (int64_t{1} << 31) && blocks < (int64_t{1} << 31), "causal_conv1d: too many workgroups (%lld)",
-                  static_cast<long long>(blocks));
+    const int64_t per_clip = sedmi::ceil_div(segments * a.vectors, kThreads);
+    SEDMI_REQUIRE(segments < (int64_t{1} << 31) && launch_ok(per_clip, kThreads), "causal_conv1d: too many workgroups per clip (%lld)",
+                  static_cast<long long>(per_clip));
     a.segments = static_cast<int>(segments), a.blocks_per_clip = static_cast<uint32_t>(per_clip);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const double items = static_cast<double>(n_clips) * frames * channels;
     sedmi::ProfileScope scope("causal_conv_kernel", st, 2.0 * width * items, 2.0 * es * items);
     return with_dtype(dtype, [&](auto t) -> int {
-        return launch_conv<decltype(t)>(width, static_cast<unsigned>(blocks), st, x, state_in, state_out, y, a);
+        using T = decltype(t);
+        const int64_t state = static_cast<int64_t>(width - 1) * channels;
+        in_launches(n_clips, per_clip, kThreads, [&](int64_t first, int64_t n) {
+            a.lengths = lengths ? lengths + first : nullptr;
+            launch_conv<T>(width, static_cast<unsigned>(n * per_clip), st, static_cast<const T *>(x) + first * x_stride_clip,
+                           state_in ? static_cast<const T *>(state_in) + first * state : nullptr,
+                           state_out ? static_cast<T *>(state_out) + first * state : nullptr,
+                           static_cast<T *>(y) + first * frames * channels, a);
+        });
+        SEDMI_CHECK_LAUNCH();
+        return SEDMI_OK;
     });
 }
 

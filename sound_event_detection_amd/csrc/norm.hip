@@ -394,7 +394,7 @@ int dtype_vec(int dtype) { return dtype == SEDMI_DTYPE_F32 ? 4 : 8; }
 bool use_slab(int64_t clips, int64_t rows, int channels, int groups, int vec) {
     const int per_group = channels / groups;
     const int64_t vectors = rows * sedmi::ceil_div(per_group, vec);
-    return per_group >= vec && (vectors <= 4096 || (vectors <= 8192 && clips * groups >= 256));
+    return per_group >= vec && launch_ok(groups, 1024) && (vectors <= 4096 || (vectors <= 8192 && clips * groups >= 256));
 }
 
 template <typename T>
@@ -403,14 +403,19 @@ void launch_slab(const T *x, T *y, NormArgs a, int64_t clips, int activation, hi
     a.per_row_inverse = a.vectors > 1 ? static_cast<uint32_t>((uint64_t{1} << 32) / a.vectors + 1) : 0;
     const int64_t vectors = a.rows * a.vectors;
     const int threads = vectors <= 512 ? 256 : vectors <= 1024 ? 512 : 1024;       // up to 2 vectors each, then up to 8
-    const unsigned blocks = static_cast<unsigned>(clips * a.groups);
-    with_activation(activation, [&](auto act) {
-        constexpr int kAct = decltype(act)::value;
-        const int64_t each = sedmi::ceil_div(vectors, threads);
-        if (each <= 1) norm_slab_kernel<T, 1, kAct><<<blocks, threads, 0, st>>>(x, y, a);
-        else if (each <= 2) norm_slab_kernel<T, 2, kAct><<<blocks, threads, 0, st>>>(x, y, a);
-        else if (each <= 4) norm_slab_kernel<T, 4, kAct><<<blocks, threads, 0, st>>>(x, y, a);
-        else norm_slab_kernel<T, 8, kAct><<<blocks, threads, 0, st>>>(x, y, a);
+    const int64_t each = sedmi::ceil_div(vectors, threads), clip = a.rows * a.channels;
+    in_launches(clips, a.groups, threads, [&](int64_t first, int64_t n) {
+        const unsigned blocks = static_cast<unsigned>(n * a.groups);
+        with_activation(activation, [&](auto act) {
+            constexpr int kAct = decltype(act)::value;
+            const T *px = x + first * clip;
+            T *py = y + first * clip;
+            if (each <= 1) norm_slab_kernel<T, 1, kAct><<<blocks, threads, 0, st>>>(px, py, a);
+            else if (each <= 2) norm_slab_kernel<T, 2, kAct><<<blocks, threads, 0, st>>>(px, py, a);
+            else if (each <= 4) norm_slab_kernel<T, 4, kAct><<<blocks, threads, 0, st>>>(px, py, a);
+            else norm_slab_kernel<T, 8, kAct><<<blocks, threads, 0, st>>>(px, py, a);
+        });
+        if (a.lengths) a.lengths += n;
     });
 }
 
@@ -452,7 +457,6 @@ int sedmi_group_norm(const void *x, const float *weight, const float *bias, cons
     const double items = static_cast<double>(n_clips) * a.rows * channels;
     const double es = dtype == SEDMI_DTYPE_F32 ? 4 : 2;
     if (use_slab(n_clips, a.rows, channels, groups, dtype_vec(dtype))) {
-        SEDMI_REQUIRE(n_clips * groups < (int64_t{1} << 31), "group_norm: too many workgroups");
         sedmi::ProfileScope scope("norm_slab_kernel", st, 8 * items, 2 * es * items);
         with_dtype(dtype, [&](auto t) -> int {
             launch_slab(static_cast<const decltype(t) *>(x), static_cast<decltype(t) *>(y), a, n_clips, activation, st);
@@ -464,31 +468,31 @@ int sedmi_group_norm(const void *x, const float *weight, const float *bias, cons
     const NormPlan p = norm_plan(n_clips, a.rows, channels, groups, dtype_vec(dtype));
     a.groups_per_block = p.groups_per_block, a.wider_blocks = p.wider_blocks, a.column_blocks = p.column_blocks;
     a.chunks = p.chunks, a.rows_per_chunk = p.rows_per_chunk;
-    const int64_t blocks = n_clips * p.chunks * p.column_blocks;
-    SEDMI_REQUIRE(blocks < (int64_t{1} << 31), "group_norm: too many workgroups (%lld)", static_cast<long long>(blocks));
+    const int64_t per_clip = static_cast<int64_t>(p.chunks) * p.column_blocks;       // at most 2^8 * 2^14
     const size_t need = static_cast<size_t>(n_clips) * p.chunks * groups * 3 * sizeof(float);
     if (ws == nullptr || ws_bytes < need)
         return sedmi::set_error(SEDMI_ENOMEM, "group_norm: workspace of %zu bytes, %zu needed", ws_bytes, need);
-    a.partial = static_cast<float *>(ws);
-    const unsigned grid = static_cast<unsigned>(blocks);
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        const T *px = static_cast<const T *>(x);
-        T *py = static_cast<T *>(y);
-        {
-            sedmi::ProfileScope scope("norm_stats_kernel", st, 4 * items, es * items);
-            if (p.tiny) norm_stats_kernel<T, true><<<grid, kThreads, 0, st>>>(px, a);
-            else norm_stats_kernel<T, false><<<grid, kThreads, 0, st>>>(px, a);
-        }
-        SEDMI_CHECK_LAUNCH();
-        {
-            sedmi::ProfileScope scope("norm_apply_kernel", st, 4 * items, 2 * es * items);
+        in_launches(n_clips, per_clip, kThreads, [&](int64_t first, int64_t n) {
+            const unsigned grid = static_cast<unsigned>(n * per_clip);
+            const T *px = static_cast<const T *>(x) + first * a.rows * channels;
+            T *py = static_cast<T *>(y) + first * a.rows * channels;
+            const double share = static_cast<double>(n) / n_clips;
+            a.lengths = lengths ? lengths + first : nullptr;
+            a.partial = static_cast<float *>(ws) + first * p.chunks * groups * 3;
+            {
+                sedmi::ProfileScope scope("norm_stats_kernel", st, share * 4 * items, share * es * items);
+                if (p.tiny) norm_stats_kernel<T, true><<<grid, kThreads, 0, st>>>(px, a);
+                else norm_stats_kernel<T, false><<<grid, kThreads, 0, st>>>(px, a);
+            }
+            sedmi::ProfileScope scope("norm_apply_kernel", st, share * 4 * items, share * 2 * es * items);
             with_activation(activation, [&](auto act) {
                 constexpr int kAct = decltype(act)::value;
                 if (p.tiny) norm_apply_kernel<T, true, kAct><<<grid, kThreads, 0, st>>>(px, py, a);
                 else norm_apply_kernel<T, false, kAct><<<grid, kThreads, 0, st>>>(px, py, a);
             });
-        }
+        });
         SEDMI_CHECK_LAUNCH();
         return SEDMI_OK;
     });

@@ -510,6 +510,19 @@ ScanArgs scan_args(const sedmi_scan_args *p) {
     return a;
 }
 
+// The arguments for the clips from `first` on.
+template <typename T>
+ScanArgs scan_args(ScanArgs a, int64_t first) {
+    const auto move = [&](const void *&p, int64_t stride) { if (p) p = static_cast<const T *>(p) + first * stride; };
+    move(a.x, a.x_clip), move(a.dt, a.dt_clip), move(a.z, a.z_clip), move(a.B, a.b_clip), move(a.C, a.c_clip);
+    a.y = static_cast<T *>(a.y) + first * a.frames * a.channels;
+    const int64_t state = first * a.channels * a.states;
+    if (a.state_in) a.state_in += state;
+    if (a.state_out) a.state_out += state;
+    if (a.lengths) a.lengths += first;
+    return a;
+}
+
 template <typename T, bool END>
 void launch_scan(int states, int waves, unsigned blocks, hipStream_t st, const ScanArgs &a) {
     if (waves == 1) {
@@ -564,21 +577,25 @@ int sedmi_selective_scan(const sedmi_scan_args *p, void *ws, size_t ws_bytes, vo
         return sedmi::set_error(SEDMI_ENOMEM, "selective_scan: workspace of %zu bytes, %zu needed", ws_bytes, need);
     a.end_state = static_cast<float *>(ws);
     a.end_step = a.end_state + static_cast<size_t>(p->n_clips) * (a.splits - 1) * p->channels * p->states;
-    const int64_t blocks = p->n_clips * blocks_of(p->channels, p->groups, 16 * waves);
-    SEDMI_REQUIRE(blocks * a.splits < (int64_t{1} << 31), "selective_scan: too many workgroups");
+    const int64_t per_clip = blocks_of(p->channels, p->groups, 16 * waves);
+    SEDMI_REQUIRE(launch_ok(per_clip * a.splits, 64 * waves), "selective_scan: too many workgroups per clip");
     hipStream_t st = static_cast<hipStream_t>(stream);
     const double items = static_cast<double>(p->n_clips) * p->frames * p->channels;
     const double es = p->dtype == SEDMI_DTYPE_F32 ? 4 : 2;
     return with_dtype(p->dtype, [&](auto t) -> int {
         using T = decltype(t);
-        if (a.splits > 1) {
-            sedmi::ProfileScope scope("selective_scan_end_kernel", st, 5 * items * p->states, 2 * es * items);
-            launch_scan<T, true>(p->states, waves, static_cast<unsigned>(blocks * (a.splits - 1)), st, a);
+        if (a.splits > 1) {                                      // few workgroups: one launch each
+            {
+                sedmi::ProfileScope scope("selective_scan_end_kernel", st, 5 * items * p->states, 2 * es * items);
+                launch_scan<T, true>(p->states, waves, static_cast<unsigned>(p->n_clips * per_clip * (a.splits - 1)), st, a);
+            }
+            SEDMI_CHECK_LAUNCH();
         }
-        SEDMI_CHECK_LAUNCH();
         {
             sedmi::ProfileScope scope("selective_scan_kernel", st, 7 * items * p->states, (p->z ? 4 : 3) * es * items);
-            launch_scan<T, false>(p->states, waves, static_cast<unsigned>(blocks * a.splits), st, a);
+            in_launches(p->n_clips, per_clip * a.splits, 64 * waves, [&](int64_t first, int64_t n) {
+                launch_scan<T, false>(p->states, waves, static_cast<unsigned>(n * per_clip * a.splits), st, scan_args<T>(a, first));
+            });
         }
         SEDMI_CHECK_LAUNCH();
         return SEDMI_OK;
@@ -595,7 +612,7 @@ int sedmi_selective_step(const sedmi_scan_args *p, void *stream) {
     ScanArgs a = scan_args(p);
     a.blocks_per_group = static_cast<int>(sedmi::ceil_div(a.per_group, kStepChannels));
     const int64_t per_clip = blocks_of(p->channels, p->groups, kStepChannels), blocks = p->n_clips * per_clip;
-    SEDMI_REQUIRE(blocks < (int64_t{1} << 31), "selective_step: too many workgroups");
+    SEDMI_REQUIRE(launch_ok(per_clip, kThreads), "selective_step: too many workgroups per stream");
     hipStream_t st = static_cast<hipStream_t>(stream);
     const double items = static_cast<double>(p->n_clips) * p->channels;
     sedmi::ProfileScope scope("selective_step_kernel", st, 7 * items * p->states, 8 * items * p->states);
@@ -605,10 +622,13 @@ int sedmi_selective_step(const sedmi_scan_args *p, void *stream) {
     const bool four = blocks >= 2048 && p->states <= 32;
     return with_dtype(p->dtype, [&](auto t) -> int {
         using T = decltype(t);
-        if (four)
-            launch_step<T, 4>(p->states, static_cast<unsigned>(sedmi::ceil_div(p->n_clips, 4) * per_clip), st, a, p->state_out, p->n_clips);
-        else
-            launch_step<T, 1>(p->states, static_cast<unsigned>(blocks), st, a, p->state_out, p->n_clips);
+        const int64_t each = four ? 4 : 1;                       // streams of a workgroup
+        in_launches(sedmi::ceil_div(p->n_clips, each), per_clip, kThreads, [&](int64_t first, int64_t n) {
+            const ScanArgs part = scan_args<T>(a, first * each);
+            const int64_t streams = std::min(n * each, p->n_clips - first * each);
+            if (four) launch_step<T, 4>(p->states, static_cast<unsigned>(n * per_clip), st, part, part.state_out, streams);
+            else launch_step<T, 1>(p->states, static_cast<unsigned>(n * per_clip), st, part, part.state_out, streams);
+        });
         SEDMI_CHECK_LAUNCH();
         return SEDMI_OK;
     });

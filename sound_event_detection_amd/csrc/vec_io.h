@@ -154,6 +154,19 @@ inline bool overlap(const void *p, const void *q, size_t bytes) {
     return p != nullptr && q != nullptr && x < y + bytes && y < x + bytes;
 }
 
+// A launch has fewer than 2^32 lanes: HIP counts them in 32 bits.
+constexpr int64_t kMaxLanes = (int64_t{1} << 32) - 1;
+
+inline bool launch_ok(int64_t blocks, int threads) { return blocks <= kMaxLanes / threads; }
+
+// Calls f(first clip, clips) for as many clips at a time as a launch of that many workgroups each can hold; a single clip's
+// have to be launch_ok.
+template <typename F>
+void in_launches(int64_t clips, int64_t blocks_per_clip, int threads, F f) {
+    const int64_t most = kMaxLanes / threads / blocks_per_clip;
+    for (int64_t first = 0; first < clips; first += most) f(first, std::min(most, clips - first));
+}
+
 // Dispatches f(T{}) on a SEDMI_DTYPE_* code.
 template <typename F>
 int with_dtype(int dtype, F f) {

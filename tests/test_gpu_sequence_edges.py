@@ -17,3 +17,57 @@ def test_group_norm_of_very_many_narrow_groups(seq, dtype, c, groups):
     _, depth = edges.two_launch_depth(1, 3, c, groups, dtype)
     y, bound = edges.group_norm(x, groups, w, b, 1e-3, depth)
     ref.check(seq.group_norm(x.cuda(), groups, w.cuda(), b.cuda(), eps=1e-3), y, bound)
+
+
+# ------------------------------------------------------------------------------- more work items than one launch can have
+def repeats(y, base):
+    """Whether the rows of y are those of base again and again, compared a part at a time."""
+    n = base.shape[0]
+    return all(bool((part.view(-1, *base.shape) == base).all()) for part in y.split(n << 10))
+
+
+def test_group_norm_of_more_groups_than_a_launch_holds(seq):
+    n, c, groups = 1 << 18, 1024, 64                               # 2^24 workgroups of 256 threads
+    base, w, b = rand(110, 64, c, dtype=F16), rand(111, c, offset=1.0), rand(112, c)
+    y, bound = ref.group_norm(base, groups, w, b, activation="silu")
+    got = seq.group_norm(base.cuda().repeat(n // 64, 1), groups, w.cuda(), b.cuda(), activation="silu")
+    ref.check(got[:64], y, bound)
+    assert repeats(got, got[:64])
+    lengths = torch.ones(n, dtype=torch.int64, device="cuda")
+    lengths[-3:] = 0
+    got = seq.group_norm(base.cuda().repeat(n // 64, 1)[:, None], groups, w.cuda(), b.cuda(), activation="silu", lengths=lengths)
+    ref.check(got[:64, 0], y, bound)
+    ref.check(got[-64:-3, 0], y[:-3], bound[:-3])
+    assert not bool(got[-3:].any())
+
+
+def test_causal_conv_of_more_clips_than_a_launch_holds(seq):
+    n, c, k = 1 << 22, 6152, 2                                     # 4 workgroups a clip; one row of x for all
+    x, w = rand(113, 1, 1, c, dtype=F16), rand(115, c, k)
+    got = seq.causal_conv1d(x.cuda().expand(n, 1, c), w.cuda())
+    y, bound, _ = ref.causal_conv1d(x, w)
+    ref.check(got[:1], y, bound)
+    assert all(bool((part == got[0]).all()) for part in got.split(1 << 18))
+
+
+def test_scan_of_more_clips_than_a_launch_holds(seq):
+    n, c, m = 1 << 22, 4, 17                                       # 4 groups of one channel: 4 workgroups a clip
+    d = scan_inputs(116, 16, 1, c, m, 4, F16)
+    y, bound, _, _ = ref.selective_scan(**d, dt_softplus=True)
+    big = {k: v if k in ("A", "D", "dt_bias") else v.repeat(n // 16, *[1] * (v.dim() - 1)) for k, v in on_gpu(d).items()}
+    got = seq.selective_scan(**big, dt_softplus=True)
+    ref.check(got[:16], y, bound)
+    assert repeats(got, got[:16])
+
+
+def test_step_of_more_streams_than_a_launch_holds(seq):
+    n, c, m = 1 << 22, 4, 33
+    d, state = scan_inputs(117, 16, None, c, m, 4, F16), rand(118, 16, c, m)
+    one = {k: v if k in ("A", "D", "dt_bias") else v[:, None] for k, v in d.items()}
+    y, bound, end, end_bound = ref.selective_scan(**one, dt_softplus=True, state=state)
+    big = {k: v if k in ("A", "D", "dt_bias") else v.repeat(n // 16, *[1] * (v.dim() - 1)) for k, v in on_gpu(d).items()}
+    held = state.cuda().repeat(n // 16, 1, 1)
+    got = seq.selective_step(**big, state=held, dt_softplus=True)
+    ref.check(got[:16], y[:, 0], bound[:, 0])
+    ref.check(held[:16], end, end_bound, "state")
+    assert repeats(got, got[:16]) and repeats(held, held[:16])
