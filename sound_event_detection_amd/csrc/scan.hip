@@ -95,7 +95,7 @@ template <typename T, int NP, bool END, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void selective_scan_kernel(ScanArgs a) {
     constexpr int kThreads = 64 * WAVES, kChannels = 16 * WAVES;
     constexpr int kYStride = kChannels + 16;                     // rows of y that a wave writes together: different banks
-    constexpr int N4 = 4 * NP;                                   // states staged per frame, zero beyond a.states
+    constexpr int N4 = 4 * NP;                                   // states staged per frame, those past a.states copies of the last
     constexpr bool kMatrix = NP >= 4;
     constexpr int kBRows = kThreads / N4 < kTile ? kThreads / N4 : kTile;    // rows of B that the workgroup loads at a time
     constexpr int kB = kTile / kBRows;
@@ -137,6 +137,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void selective_scan_kernel(ScanArgs 
     T *py = static_cast<T *>(a.y) + (clip * a.frames + row0) * a.channels + c0;
     const int64_t ox = sr * sx + pair, od = sr * sd + pair, oz = sr * sz + pair, oy = sr * sy + sc;
     const int br = min(tid / N4, kTile - 1), bn = tid % N4, bl = min(bn, a.states - 1);
+    // A state past the last is a copy of it, and C is shared out among the last and its copies in powers of two, exactly: a
+    // state of zeros would turn an infinite input into 0 * inf = NaN and pass that on to y.
+    const int copies = N4 - a.states, copy = bn - (a.states - 1);
+    const float c_share = copy < 0 ? 1.0f : __builtin_amdgcn_ldexpf(1.0f, -min(copy + 1, copies));
     const int64_t ob = br * sb + bl, oc = br * sv + bl;
     const bool gate = !END && a.z != nullptr;
     float bias[2], skip[2];
@@ -147,28 +151,24 @@ __global__ __launch_bounds__(64 * WAVES, 2) void selective_scan_kernel(ScanArgs 
         skip[e] = !END && a.D ? a.D[c] : 0.0f;
     }
 
-    // compute: a lane past the last channel repeats it, a state past the last has rate, input and output zero
+    // compute: a lane past the last channel repeats it
     const int lane = tid & 63, q = (lane >> 2) & 3;
     const int ch = (tid >> 6) * 16 + (lane >> 4) * 4 + (lane & 3);
     const bool live = ch < width;
     const int cl = c0 + min(ch, width - 1);
     auto state_of = [&](int j) __attribute__((always_inline)) { return kMatrix ? 16 * (j / 4) + 4 * q + j % 4 : q * NP + j; };
     float rate[NP], h[NP], total = 0.0f;
+    const float last_rate = decay_rate(a.A[static_cast<int64_t>(cl) * a.states + a.states - 1]);
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-        const int n = state_of(j);
-        const float v = a.A[static_cast<int64_t>(cl) * a.states + min(n, a.states - 1)];
-        rate[j] = n < a.states ? decay_rate(v) : 0.0f;
+        const float v = a.A[static_cast<int64_t>(cl) * a.states + min(state_of(j), a.states - 1)];
+        rate[j] = state_of(j) < a.states ? decay_rate(v) : last_rate;    // v without the choice: 14 registers more at 64 states
         h[j] = 0.0f;
     }
     if (!END) {
         if (a.state_in != nullptr) {
 #pragma unroll
-            for (int j = 0; j < NP; ++j) {
-                const int n = state_of(j);
-                const float v = a.state_in[(clip * a.channels + cl) * a.states + min(n, a.states - 1)];
-                h[j] = n < a.states ? v : 0.0f;
-            }
+            for (int j = 0; j < NP; ++j) h[j] = a.state_in[(clip * a.channels + cl) * a.states + min(state_of(j), a.states - 1)];
         }
         for (int s = 0; s < split; s += kJoin) {                 // the runs before this one, joined
             float d[kJoin], e[kJoin][NP];
@@ -184,7 +184,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void selective_scan_kernel(ScanArgs 
                 if (s + k >= split) break;
 #pragma unroll
                 for (int j = 0; j < NP; ++j)
-                    h[j] = fmaf(__builtin_amdgcn_exp2f(d[k] * rate[j]), h[j], state_of(j) < a.states ? e[k][j] : 0.0f);
+                    h[j] = fmaf(__builtin_amdgcn_exp2f(d[k] * rate[j]), h[j], e[k][j]);
             }
         }
     }
@@ -247,10 +247,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void selective_scan_kernel(ScanArgs 
 #pragma unroll
         for (int i = 0; i < kB; ++i) {
             const int r = br + i * kBRows;
-            const bool on = bn < a.states && (decltype(whole)::value || r < left);
+            const bool on = decltype(whole)::value || r < left;
             if (kB > 1 || tid / N4 < kTile) {
                 s_b[r][bn] = on ? static_cast<float>(rb[i]) : 0.0f;
-                if (!END) s_c[r][bn] = on ? static_cast<float>(rc[i]) : 0.0f;
+                if (!END) s_c[r][bn] = on ? static_cast<float>(rc[i]) * c_share : 0.0f;
             }
         }
     };
@@ -270,7 +270,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void selective_scan_kernel(ScanArgs 
         else if (a.softplus) stage(std::false_type{}, std::true_type{}, left);
         else stage(std::false_type{}, std::false_type{}, left);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) cx[i] = rx[i], cz[i] = second_first(rz[i], second);
+        for (int i = 0; i < 4; ++i) {
+            cx[i] = a.D ? rx[i] : Pack<T, 2>::zero();            // without D an infinite x must not meet a factor of zero
+            cz[i] = second_first(rz[i], second);
+        }
         __syncthreads();
         if (t + kTile < count) fetch_any(left_at(t + kTile));
         float *y_at = y_base;

@@ -71,3 +71,33 @@ def test_step_of_more_streams_than_a_launch_holds(seq):
     ref.check(got[:16], y[:, 0], bound[:, 0])
     ref.check(held[:16], end, end_bound, "state")
     assert repeats(got, got[:16]) and repeats(held, held[:16])
+
+
+# ------------------------------------------------------------------------------------------------- infinities in the scan
+def positive_scan(seed, n, t, c, m, dtype):
+    """Inputs whose sums over states have terms of one sign, so that an infinite input gives an infinite output."""
+    d = scan_inputs(seed, n, t, c, m, 1, dtype)
+    return {k: v if k in ("A", "dt", "dt_bias") else v.abs() for k, v in d.items()}
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("what", ["x", "dt"])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 7, 12, 16, 17, 33, 100])
+def test_scan_infinite_input_gives_infinite_output(seq, m, what, dtype):
+    # state counts between those that the lanes hold: what stands in the places left over must not reach the output
+    d = positive_scan(120, 2, 40, 19, m, dtype)
+    d[what][1, 7, 3] = float("inf")
+    for skip in (d["D"], None):
+        d["D"] = skip
+        y, bound, end, end_bound = ref.selective_scan(**d, dt_softplus=True)
+        if skip is None:
+            y[1, 7, 3] = float("inf")                              # the oracle's 0 * inf of the missing D
+        assert bool(torch.isinf(y[1, 7:, 3]).all()) and bool(torch.isinf(end[1, 3]).all())
+        got, last = seq.selective_scan(**on_gpu(d), dt_softplus=True, return_state=True)
+        ref.check(got, y, bound)
+        ref.check(last, end, end_bound, "state")
+        state = torch.zeros(2, 19, m, device="cuda")
+        one = {k: v if v is None or k in ("A", "D", "dt_bias") else v[:, 7].contiguous() for k, v in d.items()}
+        got = seq.selective_step(**on_gpu(one), state=state, dt_softplus=True)
+        assert float(got[1, 3]) == float("inf") and bool(torch.isinf(state[1, 3]).all())
+        assert int(torch.isfinite(got).sum()) == got.numel() - 1
