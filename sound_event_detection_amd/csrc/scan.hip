@@ -183,8 +183,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void selective_scan_kernel(ScanArgs 
             for (int k = 0; k < kJoin; ++k) {
                 if (s + k >= split) break;
 #pragma unroll
-                for (int j = 0; j < NP; ++j)
-                    h[j] = fmaf(__builtin_amdgcn_exp2f(d[k] * rate[j]), h[j], e[k][j]);
+                for (int j = 0; j < NP; ++j) {
+                    // half of the run's decay, twice: a growing state's 2^184 has no float32 (it made 0 into NaN), and an
+                    // infinite state is not multiplied by zero
+                    const float half = __builtin_amdgcn_exp2f(__builtin_amdgcn_fmed3f(0.5f * d[k] * rate[j], -126.0f, 127.0f));
+                    h[j] = fmaf(half, half * h[j], e[k][j]);
+                }
             }
         }
     }

@@ -101,3 +101,43 @@ def test_scan_infinite_input_gives_infinite_output(seq, m, what, dtype):
         got = seq.selective_step(**on_gpu(one), state=state, dt_softplus=True)
         assert float(got[1, 3]) == float("inf") and bool(torch.isinf(state[1, 3]).all())
         assert int(torch.isfinite(got).sum()) == got.numel() - 1
+
+
+# ---------------------------------------------------------------------------------------------- runs of a long time axis
+def is_split(n, t, c, groups, m):
+    from sound_event_detection_amd import _lib
+    return _lib.lib().sedmi_selective_scan_workspace_bytes(n, t, c, groups, m) > 0
+
+
+def test_joined_runs_of_growing_states(seq):
+    # rates above zero: a run's growth 2^184 has no float32, what it multiplies has
+    n, t, c, m = 1, 300, 24, 4
+    assert is_split(n, t, c, 1, m)
+    d = positive_scan(130, n, t, c, m, F32)
+    d["dt"], d["dt_bias"], d["z"] = torch.ones(n, t, c), None, None
+    d["A"] = torch.full((c, m), 2.0)
+    d["x"][:, :290] = 0.0                                          # no state until the last frames
+    y, bound, end, end_bound = ref.selective_scan(**d)
+    got, last = seq.selective_scan(**on_gpu(d), return_state=True)
+    ref.check(got, y, bound)
+    ref.check(last, end, end_bound, "state")
+    state = torch.full((n, c, m), 2.0 ** -120)                     # ends at 2^110 after 80 frames
+    y, bound, end, end_bound = ref.selective_scan(**d, state=state, lengths=[80])
+    got, last = seq.selective_scan(**on_gpu(d), state=state.cuda(), lengths=[80], return_state=True)
+    assert bool(torch.isfinite(end).all()) and float(end.max()) > 2.0 ** 100
+    ref.check(got, y, bound)
+    ref.check(last, end, end_bound, "state")
+
+
+def test_joined_runs_of_an_infinite_state(seq):
+    # an infinite state stays infinite, also where a run's decay is below every float32
+    n, t, c, m = 2, 300, 24, 4
+    assert is_split(n, t, c, 1, m)
+    d = positive_scan(131, n, t, c, m, F32)
+    d["A"] = torch.full((c, m), -8.0)
+    d["x"][1, 5, 3] = float("inf")
+    y, bound, end, end_bound = ref.selective_scan(**d, dt_softplus=True)
+    assert bool(torch.isinf(y[1, 5:, 3]).all())
+    got, last = seq.selective_scan(**on_gpu(d), dt_softplus=True, return_state=True)
+    ref.check(got, y, bound)
+    ref.check(last, end, end_bound, "state")
