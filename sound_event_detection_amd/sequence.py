@@ -21,12 +21,13 @@ not contiguous).  ``lengths`` gives the valid frames of each clip (an int tensor
 0 .. frames are taken as the nearer end): frames behind them are never read and come out as zeros.  An int64 tensor on
 the device is used as it is; anything else is copied there first, which waits for the copy and cannot be captured into
 a graph.  ``reverse=True`` runs from a clip's last valid frame to its first, the second direction of a bidirectional
-layer.  Nothing is kept between calls; all work goes to the current stream of the tensors' device, and apart from that
-copy nothing waits for it.
+layer.  Tensors that require a gradient (while gradients are recorded) or carry a tangent are refused.  Nothing is kept
+between calls; all work goes to the current stream of the tensors' device, and apart from that copy nothing waits for it.
 """
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -49,6 +50,10 @@ def _refuse_grad(who, *tensors):
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError(f"{who} is inference-only: call it under torch.no_grad() or on detached tensors")
+    if forward_ad._current_level >= 0:                 # within a dual_level, which no_grad() does not end
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{who} is inference-only: it has no forward derivative either, unpack the dual tensors")
 
 
 def _activation(name, who):

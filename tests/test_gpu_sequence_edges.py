@@ -141,3 +141,24 @@ def test_joined_runs_of_an_infinite_state(seq):
     got, last = seq.selective_scan(**on_gpu(d), dt_softplus=True, return_state=True)
     ref.check(got, y, bound)
     ref.check(last, end, end_bound, "state")
+
+
+# ------------------------------------------------------------------------------------------------------ forward derivatives
+def test_calls_refuse_tensors_with_a_tangent(seq):
+    from torch.autograd import forward_ad
+    x, w = torch.ones(2, 5, 8, device="cuda"), torch.ones(8, 4, device="cuda")
+    d = on_gpu(scan_inputs(140, 2, 5, 8, 4, 1, F32))
+    one = {k: v if k in ("A", "D", "dt_bias") else v[:, 0] for k, v in d.items()}
+    conv_state, scan_state = torch.zeros(2, 3, 8, device="cuda"), torch.zeros(2, 8, 4, device="cuda")
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: seq.group_norm(dual(x), 2), lambda: seq.group_norm(x, 2, bias=dual(w[:, 0])),
+                     lambda: seq.causal_conv1d(x, dual(w)), lambda: seq.causal_conv1d_step(x[:, 0], dual(conv_state), w),
+                     lambda: seq.selective_scan(**{**d, "dt": dual(d["dt"])}),
+                     lambda: seq.selective_scan(**{**d, "A": dual(d["A"])}),
+                     lambda: seq.selective_step(**one, state=dual(scan_state))):
+            with pytest.raises(RuntimeError, match="inference-only"):
+                call()
+        assert seq.group_norm(x, 2).shape == x.shape               # others are served
+    assert not bool(conv_state.any()) and not bool(scan_state.any())

@@ -1,4 +1,8 @@
 """Parts of the sequence operators that no device is needed for."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
 import test_sequence_cpu as cpu
 from test_sequence_cpu import lib  # noqa: F401  (fixture)
 
@@ -10,3 +14,18 @@ def test_a_clip_that_no_launch_can_hold_is_refused(lib):
     assert scan(lib.sedmi_selective_step, states=4, state_in=8192, state_out=8192) == -1
     assert b"workgroups" in lib.sedmi_last_error()
     assert cpu.conv(lib, clips=1, frames=1 << 38, channels=1) == -1 and b"workgroups" in lib.sedmi_last_error()
+
+
+def test_tensors_with_a_tangent_are_refused():
+    from sound_event_detection_amd import sequence
+    x = torch.ones(3)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(3))
+        sequence._refuse_grad("the call", x, None)
+        with pytest.raises(RuntimeError, match="the call is inference-only"):
+            sequence._refuse_grad("the call", x, None, dual)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="the call is inference-only"):
+            sequence._refuse_grad("the call", dual)                # no_grad leaves forward mode on
+        with torch.inference_mode():
+            sequence._refuse_grad("the call", dual)                # which switches it off
+    sequence._refuse_grad("the call", x)
