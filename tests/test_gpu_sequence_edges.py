@@ -162,3 +162,23 @@ def test_calls_refuse_tensors_with_a_tangent(seq):
                 call()
         assert seq.group_norm(x, 2).shape == x.shape               # others are served
     assert not bool(conv_state.any()) and not bool(scan_state.any())
+
+
+# ------------------------------------------------------------------------------------------------------- states in place
+def test_steps_count_as_changes_of_their_state(seq):
+    x, w = rand(150, 2, 8).cuda(), rand(151, 8, 4).cuda()
+    d = on_gpu(scan_inputs(152, 2, None, 8, 4, 1, F32))
+    for state, call in ((torch.zeros(2, 3, 8, device="cuda"), lambda s: seq.causal_conv1d_step(x, s, w)),
+                        (torch.zeros(2, 8, 4, device="cuda"), lambda s: seq.selective_step(**d, state=s, dt_softplus=True))):
+        factor = torch.ones_like(state, requires_grad=True)
+        out = (factor * state).sum()                               # keeps the state for its backward pass
+        call(state)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.backward()
+        before = state._version
+        call(state[:1].expand(2, -1, -1).contiguous())             # another tensor
+        assert state._version == before
+        with torch.inference_mode():
+            call(state.clone())                                    # has no versions
+            call(state)
+        assert state._version == before + 1
