@@ -126,9 +126,10 @@ def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=None,
         raise ValueError(f"group_norm: expected [clips, frames, ..., channels], got {tuple(x.shape)}")
     if lengths is not None and x.dim() < 3:
         raise ValueError("group_norm: lengths need a frame dimension behind the clips")
-    n, c, num_groups = x.shape[0], x.shape[-1], int(num_groups)
-    if num_groups < 1 or c == 0 or c % num_groups:
+    n, c, whole = x.shape[0], x.shape[-1], int(num_groups)
+    if whole != num_groups or whole < 1 or c == 0 or c % whole:
         raise ValueError(f"group_norm: {c} channels do not divide into {num_groups} groups")
+    num_groups = whole
     if not eps >= 0:
         raise ValueError("group_norm: eps must not be negative")
     act = _activation(activation, "group_norm")

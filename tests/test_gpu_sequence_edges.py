@@ -182,3 +182,13 @@ def test_steps_count_as_changes_of_their_state(seq):
             call(state.clone())                                    # has no versions
             call(state)
         assert state._version == before + 1
+
+
+# ------------------------------------------------------------------------------------------------------------- refusals
+def test_group_norm_refuses_a_fraction_of_a_group(seq):
+    x = torch.zeros(2, 5, 8, device="cuda")
+    for groups in (2.7, 8.5, "2"):
+        with pytest.raises(ValueError, match="do not divide"):
+            seq.group_norm(x, groups)
+    for groups in (2.0, torch.tensor(2)):
+        assert seq.group_norm(x, groups).shape == x.shape
