@@ -29,3 +29,8 @@ def test_tensors_with_a_tangent_are_refused():
         with torch.inference_mode():
             sequence._refuse_grad("the call", dual)                # which switches it off
     sequence._refuse_grad("the call", x)
+
+
+def test_the_package_names_the_module():
+    import sound_event_detection_amd
+    assert "sequence" in sound_event_detection_amd.__all__
