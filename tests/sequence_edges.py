@@ -68,7 +68,7 @@ def group_norm(x, groups, weight, bias, eps, depth, activation=None, lengths=Non
 
 # Groups of few channels, groups that end inside a vector, a group of whole vectors and one wider than a workgroup; the last
 # has one chunk per clip and long columns.
-FAR_SHAPES = [(2, 1500, 1, 24, 12), (2, 2500, 1, 60, 10), (2, 700, 4, 16, 2), (2, 70, 1, 5000, 1), (512, 640, 1, 30, 10)]
+FAR_SHAPES = [(2, 1500, 1, 24, 12), (2, 2500, 1, 60, 10), (2, 1200, 4, 16, 2), (2, 70, 1, 5000, 1), (512, 640, 1, 30, 10)]
 
 
 def far_input(shape):

@@ -4,7 +4,7 @@ import torch
 
 import sequence_edges as edges
 import sequence_reference as ref
-from test_gpu_sequence import BF16, F16, F32, TYPES, on_gpu, rand, scan_inputs, seq  # noqa: F401  (seq: fixture)
+from test_gpu_sequence import BF16, F16, F32, TYPES, gpu, layer, layer_weights, on_gpu, rand, scan_inputs, seq  # noqa: F401  (seq: fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -17,6 +17,61 @@ def test_group_norm_of_very_many_narrow_groups(seq, dtype, c, groups):
     _, depth = edges.two_launch_depth(1, 3, c, groups, dtype)
     y, bound = edges.group_norm(x, groups, w, b, 1e-3, depth)
     ref.check(seq.group_norm(x.cuda(), groups, w.cuda(), b.cuda(), eps=1e-3), y, bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", edges.FAR_SHAPES)
+def test_group_norm_of_rows_far_from_zero_in_two_launches(seq, shape, dtype):
+    # test_sequence_edges_cpu.py: squares about zero are off by more than this bound
+    from sound_event_detection_amd import _lib
+    n, t, inner, c, groups = shape
+    assert _lib.lib().sedmi_group_norm_workspace_bytes(n, t, inner, c, groups, TYPES.index(dtype)) > 0
+    x, w, b = edges.far_input(shape)
+    x = x.to(dtype)
+    chunks, depth = edges.two_launch_depth(n, t * inner, c, groups, dtype)
+    assert chunks > 1 or n == 512
+    y, bound = edges.group_norm(x, groups, w, b, 1e-5, depth)
+    ref.check(seq.group_norm(x.cuda(), groups, w.cuda(), b.cuda()), y, bound)
+
+
+# groups of 4097 .. 8192 vectors, eight to a thread; the second's rows end inside a vector
+SLABS = {F32: [(256, 600, 1, 32, 1), (128, 300, 2, 60, 2)], F16: [(256, 1100, 1, 32, 1), (128, 600, 2, 60, 2)]}
+SLABS[BF16] = SLABS[F16]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_group_norm_of_groups_that_fill_a_workgroup(seq, which, ragged, dtype):
+    n, t, inner, c, groups = SLABS[dtype][which]
+    each, depth = edges.one_launch_depth(t * inner, c, groups, dtype)
+    assert 4 < each <= 8
+    x = rand(104, n, t, inner, c, dtype=dtype, scale=1.3, offset=0.4)
+    x[3] += 60                                                     # far from zero
+    w, b = rand(105, c, offset=1.0), rand(106, c)
+    lengths = ([0, 1, t - 1, t, t // 2, t // 3, 7, t] * (n // 8)) if ragged else None
+    y, bound = edges.group_norm(x, groups, w, b, 1e-4, depth, "silu", lengths)
+    got = seq.group_norm(x.cuda(), groups, w.cuda(), b.cuda(), eps=1e-4, activation="silu", lengths=lengths)
+    ref.check(got, y, bound)
+
+
+# --------------------------------------------------------------------------------------------------- causal convolution
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype,n,t,c,rows", [(F32, 64, 250, 517, 16), (F32, 64, 250, 1037, 32), (BF16, 128, 251, 531, 16),
+                                              (F16, 128, 251, 1051, 32)])
+def test_causal_conv_in_long_runs(seq, dtype, n, t, c, rows, reverse):
+    vectors, length = -(-c // (4 if dtype == F32 else 8)), 8
+    while length < 32 and n * -(-t // length) * vectors > 262144:
+        length *= 2
+    assert length == rows
+    lengths = [0, 1, 2, 15, 16, 17, 33, t - 1] + [t, t // 2, t // 3, 47] * ((n - 8) // 4)
+    x, w, b, s = rand(107, n, t, c, dtype=dtype), rand(108, c, 4), rand(109, c), rand(160, n, 3, c, dtype=dtype)
+    y, bound, last = ref.causal_conv1d(x, w, b, "silu", s, lengths, reverse)
+    for i, v in enumerate(lengths):
+        x[i, v:] = float("nan")
+    got, end = seq.causal_conv1d(*gpu(x, w, b), "silu", s.cuda(), lengths, reverse, return_state=True)
+    ref.check(got, y, bound)
+    assert torch.equal(end.cpu(), last)
 
 
 # ------------------------------------------------------------------------------- more work items than one launch can have
@@ -141,6 +196,67 @@ def test_joined_runs_of_an_infinite_state(seq):
     got, last = seq.selective_scan(**on_gpu(d), dt_softplus=True, return_state=True)
     ref.check(got, y, bound)
     ref.check(last, end, end_bound, "state")
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m", [1, 2, 4, 5, 17, 32, 33, 64, 100, 128])
+def test_joined_runs_of_all_state_counts(seq, m, dtype, reverse):
+    n, t, c, lengths = 2, 300, 24, [300, 170]
+    assert is_split(n, t, c, 2, m)
+    d = scan_inputs(132, n, t, c, m, 2, dtype)
+    d["A"][:4] *= 1e-3                                             # channels that remember across the runs
+    state = rand(133, n, c, m)
+    y, bound, end, end_bound = ref.selective_scan(**d, dt_softplus=True, state=state, lengths=lengths, reverse=reverse)
+    got, last = seq.selective_scan(**on_gpu(d), dt_softplus=True, state=state.cuda(), lengths=lengths, reverse=reverse,
+                                   return_state=True)
+    ref.check(got, y, bound)
+    ref.check(last, end, end_bound, "state")
+
+
+@pytest.mark.parametrize("what", ["x", "dt", "state"])
+def test_joined_runs_keep_nan_in_its_channel(seq, what):
+    n, t, c, m = 2, 300, 24, 5
+    d, state = scan_inputs(134, n, t, c, m, 1, F32), rand(135, n, c, m)
+    if what == "state":
+        state[1, 3, 2] = float("nan")
+    else:
+        d[what][1, 100, 3] = float("nan")
+    y, bound, end, end_bound = ref.selective_scan(**d, dt_softplus=True, state=state)
+    got, last = seq.selective_scan(**on_gpu(d), dt_softplus=True, state=state.cuda(), return_state=True)
+    ref.check(got, y, bound)
+    ref.check(last, end, end_bound, "state")
+
+
+# ------------------------------------------------------------------------------------------------------------ from audio
+def test_events_from_audio_through_a_layer_of_them(seq):
+    # recordings of unequal length: mel features, a layer in both directions, frame probabilities, events
+    import numpy as np
+    from oracle import decode as odec
+    from sound_event_detection_amd import evaluation, feature_extraction, synth
+    audio = torch.from_numpy(synth.synth_clips(0, 3)).cuda()
+    x = feature_extraction.mel_features(audio, 16000, 2048, 128, 320, 640, log=True)
+    n, t, c = x.shape
+    lengths, classes = [t, 300, 77], 5
+    w, head = layer_weights(c, 16, 4), rand(170, 2 * c, classes, scale=c ** -0.5)
+    on_device = torch.tensor(lengths, device="cuda")
+    both = torch.cat([layer(seq, w, x, on_device, reverse)[0] for reverse in (False, True)], -1)
+    probs = torch.sigmoid(both @ head.cuda())
+
+    w64 = {k: v.cpu().double() for k, v in w.items()}
+    u = ref.group_norm(x.cpu(), 4, w64["norm_w"], w64["norm_b"], activation="silu", lengths=lengths)[0]
+    sides = []
+    for reverse in (False, True):
+        v = ref.causal_conv1d(u, w64["conv_w"], w64["conv_b"], "silu", lengths=lengths, reverse=reverse)[0]
+        bc = v @ w64["to_bc"]
+        sides.append(ref.selective_scan(v, v @ w64["to_dt"], w64["A"], bc[..., :16], bc[..., 16:], w64["D"], u, w64["dt_bias"],
+                                        True, lengths=lengths, reverse=reverse)[0])
+    want = torch.sigmoid(torch.cat(sides, -1) @ head.double())
+    assert float((probs.cpu().double() - want).abs().max()) < 1e-3         # the models' own bound on frame probabilities
+
+    seg, cls, on, off = evaluation.decode_recordings(probs.view(-1, classes), [t] * n, lengths)
+    events = [(i, *e) for i in range(n) for e in odec.decode_events(odec.threshold(probs[i].cpu().numpy()), lengths[i])]
+    assert len(events) > 10 and events == list(zip(*(np.asarray(v).tolist() for v in (seg, cls, on, off))))
 
 
 # ------------------------------------------------------------------------------------------------------ forward derivatives
