@@ -474,7 +474,8 @@ int sedmi_group_norm(const void *x, const float *weight, const float *bias, cons
  *              state_out == state_in is the form for one new frame per stream.
  *   reverse    nonzero: runs from the last valid frame to the first (the state then holds what comes
  *              behind the last frame)
- *   y          device [n_clips, frames, channels], contiguous; must not overlap x or the states */
+ *   y          device [n_clips, frames, channels], contiguous; must not overlap x or the states; nor may
+ *              state_out overlap x */
 int sedmi_causal_conv1d(const void *x, int64_t x_stride_clip, int64_t x_stride_frame, const float *weight,
                         const float *bias, const int64_t *lengths, const void *state_in, void *state_out, void *y,
                         int64_t n_clips, int64_t frames, int channels, int width, int activation, int reverse,

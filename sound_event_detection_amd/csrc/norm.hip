@@ -263,9 +263,11 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(const T *x, T *y, 
 //
 // x is read once and held as it is in memory; mean, then the squares about it, then the output.  Workgroups of the groups
 // of one clip follow each other on one die (blocks are dealt to the 8 dies in turn), so lines that two groups share are
-// fetched into one L2: by the counters every byte crosses HBM once each way.  Measured: groups of 32-byte rows (128 x 250 x
-// 16 x 64 f32, 8 groups) 79 us, 3.3 TB/s; of 64-byte rows (64 x 250 x 1024 bf16, 32 groups) 18 us, 3.6 TB/s.  A workgroup
-// reads, sums and writes in turn; twice the workgroups per compute unit (90 us) and a loop that loads the next group early
+// fetched into one L2: by the counters every byte is read once.  Groups of 32-byte rows (128 x 250 x 16 x 64 f32, 8 groups)
+// also write every byte once, 75 us, 3.5 TB/s.  Groups of 64-byte rows (64 x 250 x 1024 bf16, 32 groups) take 18 us,
+// 3.6 TB/s, and with half of the frames behind the lengths 15.5; they write a quarter more than the output has (40.8 of
+// 32.0 thousand KiB), with stores past L2 of half a 128-byte line each.  A workgroup reads, sums and writes in turn; twice
+// the workgroups per compute unit (90 us for the first shape) and a loop that loads the next group early into registers
 // (84 us) need more registers than there are and lose.
 template <typename T, int N, int ACT>
 __global__ __launch_bounds__(1024) void norm_slab_kernel(const T *x, T *y, NormArgs a) {

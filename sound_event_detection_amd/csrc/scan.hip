@@ -19,9 +19,11 @@ constexpr int kThreads = 256;
 // last; a workgroup owns 64 (or 16) channels of one clip.  Tiles of kTile frames go through LDS: there d and d*x are formed
 // once per (frame, channel) instead of once per lane, and the four lanes of a channel read them as broadcasts.
 //
-// The vector unit bounds it: one exponential and three products or sums per (frame, channel, state), 41 operations per
-// (frame, channel) around them.  64 x 250 x 1024 x 16 bf16: 72 us (135 MB, 26 us at the rate of a copy), of which the vector
-// unit issues for 61; 2 x 6000 x 1024 x 16 f16 in 32 runs: 103 us, 43 of them in the first pass.
+// The vector unit bounds it: per (frame, channel, state) one exponential (two issues of four cycles), two products and a
+// sum, and 41 operations per (frame, channel) around them: unpacking, softplus, the sums over the quarters, the gate.
+// 64 x 250 x 1024 x 16 bf16: 72 - 75 us (135 MB, 26 us at the rate of a copy); the counters give 36.3 million issues, 61 us,
+// of which the recurrence has 20.5 million, the exponentials alone 8.2.  2 x 6000 x 1024 x 16 f16 in 32 runs: 101 us, 44 of
+// them in the first pass.
 constexpr int kTile = 32;                // frames staged at a time
 constexpr int kStepChannels = 64;        // per workgroup of the single-frame form
 
@@ -47,7 +49,8 @@ struct ScanArgs {
 // log(1 + exp(x)) = max(x, 0) + log1p(e), e = exp(-|x|) <= 1, and log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3:
 // atanh(s) = s + s q P(q), q = s^2 <= 1/9, with P the polynomial of degree 3 that is nearest to the series
 // 1/3 + q/5 + q^2/7 + ... there (4.5e-9 of the result).  Step sizes of 1e-3 keep all their bits, which a logarithm of
-// the rounded sum 1 + e would not give them.
+// the rounded sum 1 + e would not give them.  What is lost is the rounding of the exponent's product, |x| 2^-24 of e: the
+// result is off by at most 6.1e-7 of itself for x >= -10, 1.0e-6 at -20, 1.9e-6 at -40.
 __device__ __forceinline__ float softplus(float x) {
     const float e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(x));
     const float s = e * __builtin_amdgcn_rcpf(2.0f + e), q = s * s;
@@ -474,8 +477,9 @@ int64_t scan_run(int64_t frames, int splits) {
 }
 
 // Runs of the time axis.  Splitting costs a second pass over all but the last run (0.6 of the scan itself), a launch and
-// the joining, so time is only split where workgroups are missing, down to one tile per run and up to four workgroups per
-// compute unit (16 waves).  Measured, whole against split (N = 16, us): 16 workgroups of 4 waves x 250 frames 30 / 18, 10 x 1000 103 / 22,
+// the joining, so time is only split where workgroups are missing, up to four workgroups per compute unit (16 waves).  Runs
+// are whole tiles of the same number: one each for a whole number of tiles, two where frames are left over (250 frames: 4
+// runs of 64).  Measured, whole against split (N = 16, us): 16 workgroups of 4 waves x 250 frames 30 / 18, 10 x 1000 103 / 22,
 // 64 x 250 30 / 19, 32 x 6000 605 / 107; 256 x 250 32 / 39, 384 x 1000 152 / 169; 8 x 64 10 / 12.  More than 64 runs
 // lose to the joining (4 x 6000: 64 runs 41, 94 runs 47).
 int scan_splits(int64_t clips, int64_t frames, int channels, int groups, int states) {

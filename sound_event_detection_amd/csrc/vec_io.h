@@ -105,6 +105,7 @@ __device__ __forceinline__ void stream_pack(T *p, const Pack<T, V> &r, int n) {
     }
 }
 
+// 0 from x = -87.4 down, where the reciprocal is below 2^-126 (the value is above -1.3e-36 there).
 __device__ __forceinline__ float silu(float x) { return x * __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
 
 // x Phi(x) = max(x, 0) - |x| erfc(z) / 2 with z = |x| / sqrt 2, which cancels nowhere.  erfc(z) = exp(-z^2) t Q(t),

@@ -188,7 +188,7 @@ def causal_conv1d(x, weight, bias=None, activation=None, state=None, lengths=Non
 
 def causal_conv1d_step(x, state, weight, bias=None, activation=None):
     """One new frame x [streams, channels] of every stream: the convolution's output [streams, channels], ``state``
-    [streams, width - 1, channels] (the type of x, contiguous) moved on by this frame in place."""
+    [streams, width - 1, channels] (the type of x, contiguous) moved on by this frame in place; x must not be part of it."""
     dtype = _check_input(x, "causal_conv1d_step")
     _refuse_grad("causal_conv1d_step", x, weight, bias, state)
     if x.dim() != 2 or x.shape[1] == 0:
